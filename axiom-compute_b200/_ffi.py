@@ -32,6 +32,8 @@ AXC_ERR_INVALID_ARGUMENT = 100
 AXC_FINISH_OVERLAP_PREVIOUS = 1
 AXC_FINISH_LET_NEXT_START = 2
 AXC_TY_OTHER, AXC_TY_U8, AXC_TY_F32, AXC_TY_U32 = 0, 1, 2, 3
+AXC_TY_BF16, AXC_TY_F16, AXC_TY_I32, AXC_TY_I64 = 4, 5, 6, 7
+AXC_MXFP4_MATVEC_TOKENS = 8
 AXC_ACCESS_READ_ONLY, AXC_ACCESS_READ_WRITE, AXC_ACCESS_WRITE_ONLY = 1, 2, 3
 
 
@@ -128,6 +130,17 @@ SYMBOLS = {
     "axc_cuda_q4k_prefill": (C.c_int, [_VP, _VP, _VP, C.c_uint32, C.c_uint32, C.c_uint32, _VP, _VP]),
     "axc_cuda_q4k_prefill_form": (C.c_int, [_VP, _VP, _VP, C.c_uint32, C.c_uint32, C.c_uint32, _VP, _VP, C.c_int,
                                             C.c_uint32]),
+    "axc_cuda_mxfp4_scale_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32]),
+    "axc_cuda_mxfp4_quantize": (C.c_int, [_VP, C.c_uint32, C.c_uint64, C.c_uint32, C.c_uint32, _VP, _VP, _VP]),
+    "axc_cuda_mxfp4_dequant": (C.c_int, [_VP, _VP, _VP, C.c_uint32, C.c_uint32, C.c_uint32, _VP]),
+    "axc_cuda_mxfp4_matvec": (C.c_int, [_VP, _VP, _VP, _VP, C.c_uint32, C.c_uint32, C.c_uint32, _VP, _VP]),
+    "axc_cuda_mxfp4_prefill": (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _VP, _VP]),
+    "axc_cuda_q4k_embed": (C.c_int, [_VP, _VP, C.c_uint32, C.c_uint32, _VP, C.c_uint32, C.c_uint32, C.c_uint32, C.c_float,
+                                     _VP, _VP]),
+    "axc_cuda_q4_0_embed": (C.c_int, [_VP, _VP, C.c_uint32, C.c_uint32, _VP, C.c_uint32, C.c_uint32, C.c_uint32, C.c_float,
+                                      _VP, _VP]),
+    "axc_cuda_mxfp4_embed": (C.c_int, [_VP, _VP, _VP, C.c_uint32, C.c_uint32, _VP, C.c_uint32, C.c_uint32, C.c_uint32,
+                                       C.c_float, _VP, _VP]),
     "axc_cuda_q4k_matvec_fused": (C.c_int, [_VP, C.POINTER(AxcXSrc), _VP, C.c_uint32, C.c_uint32,
                                             C.POINTER(AxcGather), _VP, _VP, C.POINTER(AxcTuning)]),
     "axc_cuda_q4k_prepared_x_bytes": (C.c_size_t, [C.c_uint32]),

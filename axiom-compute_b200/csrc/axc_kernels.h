@@ -133,4 +133,28 @@ cudaError_t launch_q4_0_matvec_seq(const uint8_t* q, const float* x, float* y, u
 cudaError_t launch_q4_0_dequant(const uint8_t* q, float* w, uint32_t rows, uint32_t n_blocks,
                                 cudaStream_t stream);
 
+// Element types of the operators that read or write more than fp32.
+enum class ElemType { F32, BF16, F16 };
+
+// x [rows][row_stride] -> MXFP4 codes and scale tiles (layout: axc_mx.cuh); the last block of a row is filled up
+// with zeros.
+cudaError_t launch_mxfp4_quantize(const void* x, ElemType type, uint64_t row_stride, uint32_t rows, uint32_t cols,
+                                  uint8_t* codes, uint8_t* scales, cudaStream_t stream);
+// out[i] = dequant(row ids[i]) * factor; ids == nullptr: all rows in order, factor unused.
+cudaError_t launch_q4k_embed(const uint8_t* q, const void* ids, int ids64, uint32_t n_ids, uint32_t rows, uint32_t n_sb,
+                             float factor, void* out, ElemType type, uint32_t* status, cudaStream_t stream);
+cudaError_t launch_q4_0_embed(const uint8_t* q, const void* ids, int ids64, uint32_t n_ids, uint32_t rows, uint32_t n_blocks,
+                              float factor, void* out, ElemType type, uint32_t* status, cudaStream_t stream);
+cudaError_t launch_mxfp4_embed(const uint8_t* codes, const uint8_t* scales, const void* ids, int ids64, uint32_t n_ids,
+                               uint32_t rows, uint32_t n_blocks, float factor, void* out, ElemType type, uint32_t* status,
+                               cudaStream_t stream);
+// y[t][r] = sum_k W[r][k] x[t][k], W in MXFP4, x and y fp32, 1..MX_MATVEC_TOKENS tokens.
+constexpr uint32_t MX_MATVEC_TOKENS = 8;
+cudaError_t launch_mxfp4_matvec(const uint8_t* codes, const uint8_t* scales, const float* x, float* y, uint32_t m_tokens,
+                                uint32_t rows, uint32_t n_blocks, uint32_t* status, cudaStream_t stream, int sm_count);
+// C[m][n] = sum_k A[m][k] W[n][k], both in MXFP4, fp32 accumulate, C in `type`.
+cudaError_t launch_mxfp4_prefill(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* a_codes,
+                                 const uint8_t* a_scales, void* c, ElemType type, uint32_t m_tokens, uint32_t n_rows,
+                                 uint32_t n_blocks, uint32_t* status, cudaStream_t stream, int sm_count);
+
 }  // namespace axc

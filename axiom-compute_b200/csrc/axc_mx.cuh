@@ -1,0 +1,60 @@
+// MXFP4 on the device: blocks of 32 E2M1 values with one E8M0 (power of two) scale.
+//
+//   codes   [rows][n_blocks * 16] bytes, element 2j of a row in the low nibble of byte j, 2j + 1 in the high one.
+//           A code is a sign bit and a magnitude 0..7 that stands for 0, 0.5, 1, 1.5, 2, 3, 4, 6.
+//   scales  one byte b per block, 2^(b - 127), 255 = NaN, in tiles of 128 rows x 4 blocks: the order in which the
+//           tensor cores' block-scaled products take them (32 lanes of 16 bytes, a lane holding the four scales of
+//           rows r, r + 32, r + 64 and r + 96).  Tiles of one row range follow one another along the blocks; rows
+//           and blocks that only fill up a tile are zero.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "axc_device.cuh"
+
+namespace axc {
+
+constexpr int MX_BLOCK = 32;          // values per scale
+constexpr int MX_BLOCK_BYTES = 16;
+constexpr uint32_t MX_TILE_ROWS = 128, MX_TILE_BLOCKS = 4, MX_TILE_BYTES = 512;
+
+__host__ __device__ __forceinline__ uint64_t mx_scale_bytes(uint64_t rows, uint64_t n_blocks) {
+    return (rows + 127u) / 128u * ((n_blocks + 3u) / 4u) * MX_TILE_BYTES;
+}
+
+// Byte offset of the scales of blocks 4 * quad .. 4 * quad + 3 of a row; n_quads = ceil(n_blocks / 4).
+__host__ __device__ __forceinline__ uint64_t mx_scale_at(uint64_t row, uint32_t quad, uint32_t n_quads) {
+    return ((row >> 7) * n_quads + quad) * MX_TILE_BYTES + (row & 31u) * 16u + ((row >> 5) & 3u) * 4u;
+}
+
+// 2^(byte - 127); 255 is NaN.
+__device__ __forceinline__ float mx_scale_value(uint32_t byte) {
+    return __int_as_float(byte == 0u ? 0x00400000 : byte == 255u ? 0x7FFFFFFF : (int)(byte << 23));
+}
+
+// The two values of one byte of codes, exactly, as fp16 (low nibble first).
+__device__ __forceinline__ float2 mx_code_pair(uint32_t byte) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 b;\n\tcvt.u8.u32 b, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(h) : "r"(byte));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// Eight consecutive output values, rounded to nearest even, in one or two 16-byte stores.
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    __nv_bfloat162 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
+__device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
+    __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
+
+}  // namespace axc

@@ -951,6 +951,134 @@ int axc_cuda_q4k_prefill_form(const void* q, const uint16_t* a_bf16, float* c, u
     return launch_result(e);
 }
 
+// ---- MXFP4 matrices and rows of quantised tables ----
+
+static bool elem_type(uint32_t code, axc::ElemType* out) {
+    switch (code) {
+        case AXC_TY_F32: *out = axc::ElemType::F32; return true;
+        case AXC_TY_BF16: *out = axc::ElemType::BF16; return true;
+        case AXC_TY_F16: *out = axc::ElemType::F16; return true;
+    }
+    return false;
+}
+
+static size_t elem_size(axc::ElemType t) { return t == axc::ElemType::F32 ? 4 : 2; }
+
+// Rows and blocks per row whose byte counts and TMA coordinates the kernels can address.
+static bool mx_shape_ok(uint32_t rows, uint32_t n_blocks) { return rows < (1u << 31) && n_blocks < (1u << 26); }
+
+size_t axc_cuda_mxfp4_scale_bytes(uint32_t rows, uint32_t n_blocks) {
+    return ((size_t)rows + 127) / 128 * (((size_t)n_blocks + 3) / 4) * 512;
+}
+
+int axc_cuda_mxfp4_quantize(const void* x, uint32_t x_type, uint64_t row_stride, uint32_t rows, uint32_t cols, void* codes,
+                            void* scales, void* stream) {
+    clear_error();
+    axc::ElemType t;
+    if (!elem_type(x_type, &t)) return fail(AXC_ERR_INVALID_ARGUMENT, "x must be fp32, bf16 or fp16");
+    if (rows == 0 || cols == 0) return AXC_OK;
+    if (!x || !codes || !scales) return fail(AXC_ERR_INVALID_ARGUMENT, "null device pointer");
+    if (((uintptr_t)codes | (uintptr_t)scales) & 15u)
+        return fail(AXC_ERR_INVALID_ARGUMENT, "device pointers must be 16-byte aligned");
+    if ((uintptr_t)x % elem_size(t)) return fail(AXC_ERR_INVALID_ARGUMENT, "x must be aligned to its elements");
+    if (rows > 1 && row_stride < cols) return fail(AXC_ERR_INVALID_ARGUMENT, "row stride %llu is less than %u columns", (unsigned long long)row_stride, cols);
+    if (cols > (1u << 31) || !mx_shape_ok(rows, cols / 32)) return fail(AXC_ERR_INVALID_ARGUMENT, "quantise shape out of range");
+    return launch_result(axc::launch_mxfp4_quantize(x, t, row_stride, rows, cols, (uint8_t*)codes, (uint8_t*)scales, (cudaStream_t)stream));
+}
+
+int axc_cuda_mxfp4_dequant(const void* codes, const void* scales, void* w, uint32_t w_type, uint32_t rows, uint32_t n_blocks,
+                           void* stream) {
+    clear_error();
+    axc::ElemType t;
+    if (!elem_type(w_type, &t)) return fail(AXC_ERR_INVALID_ARGUMENT, "w must be fp32, bf16 or fp16");
+    if (rows == 0 || n_blocks == 0) return AXC_OK;
+    int rc = check_dev_ptrs(codes, scales, w);
+    if (rc != AXC_OK) return rc;
+    if (!mx_shape_ok(rows, n_blocks)) return fail(AXC_ERR_INVALID_ARGUMENT, "dequant shape out of range");
+    return launch_result(axc::launch_mxfp4_embed((const uint8_t*)codes, (const uint8_t*)scales, nullptr, 0, rows, rows, n_blocks, 1.0f, w, t, nullptr, (cudaStream_t)stream));
+}
+
+int axc_cuda_mxfp4_matvec(const void* codes, const void* scales, const float* x, float* y, uint32_t m_tokens, uint32_t rows,
+                          uint32_t n_blocks, void* stream, uint32_t* status) {
+    clear_error();
+    if (m_tokens > AXC_MXFP4_MATVEC_TOKENS)
+        return fail(AXC_ERR_INVALID_ARGUMENT, "the MXFP4 matvec serves 1..%u tokens", (unsigned)AXC_MXFP4_MATVEC_TOKENS);
+    if (rows == 0 || m_tokens == 0) return AXC_OK;
+    if (n_blocks == 0) {
+        if (!y) return fail(AXC_ERR_INVALID_ARGUMENT, "null device pointer");
+        return launch_result(cudaMemsetAsync(y, 0, (size_t)m_tokens * rows * 4, (cudaStream_t)stream));
+    }
+    int rc = check_dev_ptrs(codes, scales, x);
+    if (rc != AXC_OK) return rc;
+    if (!y || ((uintptr_t)y & 3u)) return fail(AXC_ERR_INVALID_ARGUMENT, "y must be non-null and 4-byte aligned");
+    if (!mx_shape_ok(rows, n_blocks)) return fail(AXC_ERR_INVALID_ARGUMENT, "matvec shape out of range");
+    cudaError_t e = axc::launch_mxfp4_matvec((const uint8_t*)codes, (const uint8_t*)scales, x, y, m_tokens, rows, n_blocks, status, (cudaStream_t)stream, sm_count_of_current_device());
+    if (e == cudaErrorNotSupported)
+        return fail(AXC_ERR_PIPELINE_CREATION_FAILED, "pipeline creation failed: the driver does not provide cuTensorMapEncodeTiled");
+    return launch_result(e);
+}
+
+int axc_cuda_mxfp4_prefill(const void* w_codes, const void* w_scales, const void* a_codes, const void* a_scales, void* c,
+                           uint32_t c_type, uint32_t m_tokens, uint32_t n_rows, uint32_t n_blocks, void* stream,
+                           uint32_t* status) {
+    clear_error();
+    axc::ElemType t;
+    if (!elem_type(c_type, &t)) return fail(AXC_ERR_INVALID_ARGUMENT, "c must be fp32, bf16 or fp16");
+    if (m_tokens == 0 || n_rows == 0) return AXC_OK;
+    if (!c || (uintptr_t)c & 15u) return fail(AXC_ERR_INVALID_ARGUMENT, "c must be non-null and 16-byte aligned");
+    if (n_blocks == 0) return launch_result(cudaMemsetAsync(c, 0, (size_t)m_tokens * n_rows * elem_size(t), (cudaStream_t)stream));
+    int rc = check_dev_ptrs(w_codes, w_scales, a_codes);
+    if (rc != AXC_OK) return rc;
+    if (!a_scales || (uintptr_t)a_scales & 15u) return fail(AXC_ERR_INVALID_ARGUMENT, "device pointers must be 16-byte aligned");
+    if (!mx_shape_ok(n_rows, n_blocks) || m_tokens > (1u << 23)) return fail(AXC_ERR_INVALID_ARGUMENT, "prefill shape out of range");
+    cudaError_t e = axc::launch_mxfp4_prefill((const uint8_t*)w_codes, (const uint8_t*)w_scales, (const uint8_t*)a_codes, (const uint8_t*)a_scales, c, t, m_tokens, n_rows, n_blocks, status, (cudaStream_t)stream, sm_count_of_current_device());
+    if (e == cudaErrorNotSupported)
+        return fail(AXC_ERR_PIPELINE_CREATION_FAILED, "pipeline creation failed: the driver does not provide cuTensorMapEncodeTiled");
+    return launch_result(e);
+}
+
+static int check_embed(const void* q, const void* scales, const void* ids, uint32_t ids_type, uint32_t n_ids, const void* out,
+                       uint32_t out_type, axc::ElemType* t) {
+    if (!elem_type(out_type, t)) return fail(AXC_ERR_INVALID_ARGUMENT, "out must be fp32, bf16 or fp16");
+    if (ids_type != AXC_TY_I32 && ids_type != AXC_TY_I64) return fail(AXC_ERR_INVALID_ARGUMENT, "ids must be int32 or int64");
+    if (n_ids == 0) return AXC_OK;
+    int rc = check_dev_ptrs(q, scales, out);
+    if (rc != AXC_OK) return rc;
+    if (!ids || (uintptr_t)ids % (ids_type == AXC_TY_I64 ? 8 : 4))
+        return fail(AXC_ERR_INVALID_ARGUMENT, "ids must be non-null and aligned to their type");
+    return AXC_OK;
+}
+
+int axc_cuda_q4k_embed(const void* q, const void* ids, uint32_t ids_type, uint32_t n_ids, void* out, uint32_t out_type,
+                       uint32_t rows, uint32_t n_superblocks, float scale, void* stream, uint32_t* status) {
+    clear_error();
+    axc::ElemType t = axc::ElemType::F32;
+    int rc = n_superblocks == 0 ? check_embed(ids, ids, ids, ids_type, 0, out, out_type, &t) : check_embed(q, q, ids, ids_type, n_ids, out, out_type, &t);
+    if (rc != AXC_OK) return rc;
+    if (n_superblocks >= (1u << 23)) return fail(AXC_ERR_INVALID_ARGUMENT, "embed shape out of range");
+    return launch_result(axc::launch_q4k_embed((const uint8_t*)q, ids, ids_type == AXC_TY_I64, n_ids, rows, n_superblocks, scale, out, t, status, (cudaStream_t)stream));
+}
+
+int axc_cuda_q4_0_embed(const void* q, const void* ids, uint32_t ids_type, uint32_t n_ids, void* out, uint32_t out_type,
+                        uint32_t rows, uint32_t n_blocks, float scale, void* stream, uint32_t* status) {
+    clear_error();
+    axc::ElemType t = axc::ElemType::F32;
+    int rc = n_blocks == 0 ? check_embed(ids, ids, ids, ids_type, 0, out, out_type, &t) : check_embed(q, q, ids, ids_type, n_ids, out, out_type, &t);
+    if (rc != AXC_OK) return rc;
+    if (n_blocks >= (1u << 26)) return fail(AXC_ERR_INVALID_ARGUMENT, "embed shape out of range");
+    return launch_result(axc::launch_q4_0_embed((const uint8_t*)q, ids, ids_type == AXC_TY_I64, n_ids, rows, n_blocks, scale, out, t, status, (cudaStream_t)stream));
+}
+
+int axc_cuda_mxfp4_embed(const void* codes, const void* scales, const void* ids, uint32_t ids_type, uint32_t n_ids, void* out,
+                         uint32_t out_type, uint32_t rows, uint32_t n_blocks, float scale, void* stream, uint32_t* status) {
+    clear_error();
+    axc::ElemType t = axc::ElemType::F32;
+    int rc = n_blocks == 0 ? check_embed(ids, ids, ids, ids_type, 0, out, out_type, &t) : check_embed(codes, scales, ids, ids_type, n_ids, out, out_type, &t);
+    if (rc != AXC_OK) return rc;
+    if (n_blocks >= (1u << 26)) return fail(AXC_ERR_INVALID_ARGUMENT, "embed shape out of range");
+    return launch_result(axc::launch_mxfp4_embed((const uint8_t*)codes, (const uint8_t*)scales, ids, ids_type == AXC_TY_I64, n_ids, rows, n_blocks, scale, out, t, status, (cudaStream_t)stream));
+}
+
 int axc_cuda_q4k_matvec_fused(const void* q, const axc_xsrc* xs, float* y, uint32_t rows,
                               uint32_t n_superblocks, const axc_gather* g, void* stream,
                               uint32_t* status, const axc_tuning* tuning) {

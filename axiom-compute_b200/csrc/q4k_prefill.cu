@@ -24,14 +24,13 @@
 // Every wait on an mbarrier is bounded; a wait that runs out sets an error bit and an abort flag,
 // all roles fall through to the common exit, outstanding copies are waited for and tensor memory
 // is freed.
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
 #include <mutex>
 
 #include "axc_device.cuh"
 #include "axc_kernels.h"
+#include "axc_umma.cuh"
 
 namespace axc {
 namespace {
@@ -56,24 +55,6 @@ constexpr uint32_t PF_THREADS = (3 + PF_DEQ_WARPS) * 32;
 constexpr uint32_t PF_IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((PF_TOK >> 3) << 17) | ((PF_ROWS >> 4) << 24);
 // the pair form: M = 256 over the two CTAs
 constexpr uint32_t PF_IDESC_PAIR = (1u << 4) | (1u << 7) | (1u << 10) | ((PF_TOK >> 3) << 17) | ((256u >> 4) << 24);
-
-// Shared-memory matrix descriptor of a K-major tile whose rows are 128 bytes (64 bf16) with the
-// 128-byte swizzle: start address / 16, leading offset 1 (unused with a swizzle), stride between
-// 8-row groups 1024 B / 16, descriptor version 1, layout type 2 (128-byte swizzle).
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t smem_addr) {
-    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-            "r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 
 __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t accumulate) {
     asm volatile(
@@ -133,11 +114,6 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
 
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
 }
 
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
@@ -413,25 +389,13 @@ q4k_prefill_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }();
-    return fn;
-}
-
 }  // namespace
 
 cudaError_t launch_q4k_prefill(const uint8_t* q, const uint16_t* a_bf16, float* c, uint32_t m_tokens,
                                uint32_t n_rows, uint32_t n_sb, uint32_t* status, cudaStream_t stream, int form,
                                bool independent) {
     if (m_tokens == 0 || n_rows == 0 || n_sb == 0) return cudaSuccess;
-    auto encode = encode_fn();
+    auto encode = tensor_map_encoder();
     if (!encode) return cudaErrorNotSupported;
     const uint32_t tiles = (n_rows + PF_ROWS - 1) / PF_ROWS;
     const bool pair = form != 1 && tiles >= 2;   // form: 0 = choose, 1 = single CTA, 2 = CTA pair

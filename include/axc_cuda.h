@@ -76,6 +76,8 @@ typedef struct axc_ctx_opts {
 /* Element type / access of one buffer binding (axc-hir ScalarTy / BufferAccess,
  * crates/axc-hir/src/ty.rs:13-26, crates/axc-hir/src/buffer.rs:16-49). */
 enum { AXC_TY_U8 = 1, AXC_TY_F32 = 2, AXC_TY_U32 = 3, AXC_TY_OTHER = 0 };
+/* Further element types of the device layer (never of a binding). */
+enum { AXC_TY_BF16 = 4, AXC_TY_F16 = 5, AXC_TY_I32 = 6, AXC_TY_I64 = 7 };
 enum { AXC_ACCESS_READ_ONLY = 1, AXC_ACCESS_READ_WRITE = 2, AXC_ACCESS_WRITE_ONLY = 3 };
 
 /* One BufferBindingSlot of the ParamBindingPlan (crates/axc-hir/src/param.rs:66-78). */
@@ -306,6 +308,58 @@ int axc_cuda_q4k_prefill(const void* q, const uint16_t* a_bf16, float* c, uint32
 int axc_cuda_q4k_prefill_form(const void* q, const uint16_t* a_bf16, float* c, uint32_t m_tokens,
                               uint32_t n_rows, uint32_t n_superblocks, void* stream, uint32_t* status, int form,
                               uint32_t flags);
+
+/* ---- MXFP4: blocks of 32 four-bit values with a power-of-two scale each ----
+ *
+ * A matrix of `rows` rows of n_blocks * 32 values is two buffers in device memory, both 16-byte aligned:
+ *   codes   rows * n_blocks * 16 bytes, row after row; value 2j of a row is the low nibble of its byte j, value
+ *           2j + 1 the high one.  A nibble is a sign bit (8) and a magnitude 0..7 for 0, 0.5, 1, 1.5, 2, 3, 4, 6;
+ *   scales  axc_cuda_mxfp4_scale_bytes(rows, n_blocks) bytes: byte b of a block stands for 2^(b - 127), 255 for
+ *           NaN.  The byte of (row, block) lies at
+ *             ((row / 128) * ceil(n_blocks / 4) + block / 4) * 512 + (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4,
+ *           the order in which the tensor cores take scales; bytes that belong to no (row, block) are zero
+ *           (axc_cuda_mxfp4_quantize writes them; whoever fills the buffer otherwise must too).
+ * The reference has no such format; it stands beside its Q4_K_M and Q4_0 (examples/q4km_dequant_matvec.axc,
+ * examples/q4_0_dequant_matvec.axc). */
+size_t axc_cuda_mxfp4_scale_bytes(uint32_t rows, uint32_t n_blocks);
+/* x [rows][row_stride] (row_stride in elements, aligned to its elements; x_type AXC_TY_F32, AXC_TY_BF16 or
+ * AXC_TY_F16) to MXFP4 with ceil(cols / 32) blocks per row, the last one filled up with zeros.  Per block the scale
+ * is 2^e, e = clamp(floor(log2(max |x|)) - 2, -127, 127), and every value the nearest of the block's 15 points, ties
+ * to the even code, magnitudes above the largest point to that point.  A block that holds a NaN or an infinity gets
+ * the NaN scale and zero codes. */
+int axc_cuda_mxfp4_quantize(const void* x, uint32_t x_type, uint64_t row_stride, uint32_t rows, uint32_t cols, void* codes,
+                            void* scales, void* stream);
+/* w [rows][n_blocks * 32] = the values, exact in fp32, rounded to nearest even in bf16 / fp16. */
+int axc_cuda_mxfp4_dequant(const void* codes, const void* scales, void* w, uint32_t w_type, uint32_t rows, uint32_t n_blocks,
+                           void* stream);
+/* y[t][r] = sum_k W[r][k] * x[t][k] for m_tokens vectors x of n_blocks * 32 fp32 values, 1..8 of them.  x is not
+ * rounded to 4 bits: within each block of 32 columns it is held as an integer of 23 bits with sign, relative to the
+ * block's largest |x| (error at most 2^-22 of that), and the products with its base-8 digits are exact on the tensor
+ * cores; sums are fp32.  Blocks whose largest |x| is below 2^-105 keep the absolute resolution 2^-128.  A block of x with a NaN, an infinity or a magnitude
+ * of 2^127 or more makes every y of that token NaN.  n_blocks = 0 gives zeros.  *status (nullable) receives bit 0
+ * if a bounded wait inside the kernel ran out. */
+#define AXC_MXFP4_MATVEC_TOKENS 8
+int axc_cuda_mxfp4_matvec(const void* codes, const void* scales, const float* x, float* y, uint32_t m_tokens, uint32_t rows,
+                          uint32_t n_blocks, void* stream, uint32_t* status);
+/* C[m][n] = sum_k A[m][k] * W[n][k] on the tensor cores' block-scaled path: W (n_rows) and A (m_tokens rows) are
+ * MXFP4 matrices with n_blocks blocks per row, C is m_tokens x n_rows row-major in c_type, fp32 accumulation, one
+ * rounding to c_type.  n_blocks = 0 gives zeros.  *status as for the matvec. */
+int axc_cuda_mxfp4_prefill(const void* w_codes, const void* w_scales, const void* a_codes, const void* a_scales, void* c,
+                           uint32_t c_type, uint32_t m_tokens, uint32_t n_rows, uint32_t n_blocks, void* stream,
+                           uint32_t* status);
+
+/* ---- rows of a quantised table by number (token embedding) ----
+ *
+ * out[i] = round(dequant(row ids[i]) * scale): the fp32 values of the *_dequant calls, multiplied in fp32, rounded
+ * once to out_type.  ids: n_ids numbers of ids_type AXC_TY_I32 or AXC_TY_I64 in device memory, any order, repeats
+ * allowed.  An id outside [0, rows) (say -1 for padding) reads nothing: its row of out is zero and bit 1 (value 2)
+ * of *status (nullable) is set.  out: n_ids rows, 16-byte aligned. */
+int axc_cuda_q4k_embed(const void* q, const void* ids, uint32_t ids_type, uint32_t n_ids, void* out, uint32_t out_type,
+                       uint32_t rows, uint32_t n_superblocks, float scale, void* stream, uint32_t* status);
+int axc_cuda_q4_0_embed(const void* q, const void* ids, uint32_t ids_type, uint32_t n_ids, void* out, uint32_t out_type,
+                        uint32_t rows, uint32_t n_blocks, float scale, void* stream, uint32_t* status);
+int axc_cuda_mxfp4_embed(const void* codes, const void* scales, const void* ids, uint32_t ids_type, uint32_t n_ids, void* out,
+                         uint32_t out_type, uint32_t rows, uint32_t n_blocks, float scale, void* stream, uint32_t* status);
 
 /* Q4_K_M matvec whose activations are assembled inside the kernel: x = a [+ b], where a and b
  * are each a plain fp32 vector (x, x2) or a vector of (value, epoch) words that the all-gather
