@@ -15,7 +15,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libaxc_cuda.so")
 SOURCES = ["axc_runtime.cu", "q4_stream.cu", "q4k_matvec.cu", "q4_0_matvec.cu", "q4k_prefill.cu", "axc_static.cu",
-           "mxfp4_quantize.cu", "mxfp4_product.cu", "q4_embed.cu"]
+           "mxfp4_quantize.cu", "mxfp4_product.cu", "mxfp4_gemm.cu", "q4_embed.cu"]
 HEADERS = ["axc_device.cuh", "axc_mx.cuh", "axc_umma.cuh", "axc_kernels.h", os.path.join("..", "..", "include", "axc_cuda.h")]
 
 NVCC_FLAGS = [

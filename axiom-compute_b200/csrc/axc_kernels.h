@@ -156,5 +156,9 @@ cudaError_t launch_mxfp4_matvec(const uint8_t* codes, const uint8_t* scales, con
 cudaError_t launch_mxfp4_prefill(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* a_codes,
                                  const uint8_t* a_scales, void* c, ElemType type, uint32_t m_tokens, uint32_t n_rows,
                                  uint32_t n_blocks, uint32_t* status, cudaStream_t stream, int sm_count);
+// The form for many tokens (mxfp4_gemm.cu).
+cudaError_t launch_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* a_codes, const uint8_t* a_scales,
+                              void* c, ElemType type, uint32_t m_tokens, uint32_t n_rows, uint32_t n_blocks,
+                              uint32_t* status, cudaStream_t stream, int sm_count);
 
 }  // namespace axc

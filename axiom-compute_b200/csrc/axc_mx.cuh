@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 
 #include "axc_device.cuh"
+#include "axc_umma.cuh"
 
 namespace axc {
 
@@ -55,6 +56,29 @@ __device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
+
+// kind::mxf4 instruction descriptor: both operands E2M1 (1 at bits 7 and 10), K-major, E8M0 scales (bit 23), N >> 3 at
+// bit 17, M >> 7 at bit 27; sf_id (0 or 2: which two of a column's four scale bytes) at bits 4 and 29.
+__device__ __forceinline__ uint32_t mx_idesc(uint32_t m, uint32_t n, uint32_t sf_id) {
+    return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 7) << 27) | (sf_id << 4) | (sf_id << 29);
+}
+
+// Shared-memory descriptor of a 512-byte scale tile: 32 rows of 16 bytes, no swizzle, 8 rows 128 bytes apart.
+__device__ __forceinline__ uint64_t mx_scale_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | (8ull << 16) | (8ull << 32) | (1ull << 46);
+}
+
+// Tensor map of a matrix' codes: boxes of 256 columns (128 bytes, 128-byte swizzle) x box_rows rows; what lies outside
+// the matrix reads as zero.
+inline bool mx_encode_codes(CUtensorMap* map, const uint8_t* codes, uint32_t rows, uint32_t n_blocks, uint32_t box_rows) {
+    cuuint64_t dims[2] = {(uint64_t)n_blocks * MX_BLOCK_BYTES, rows};
+    cuuint64_t strides[1] = {(uint64_t)n_blocks * MX_BLOCK_BYTES};
+    cuuint32_t box[2] = {128u, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, estr,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace axc

@@ -1,0 +1,289 @@
+// C[m][n] = sum_k A[m][k] W[n][k] for many tokens, A and W in MXFP4: the form of axc_cuda_mxfp4_prefill that is
+// bound by the tensor cores (tcgen05.mma kind::mxf4, block scales, fp32 accumulators in tensor memory).
+//
+// A pair of CTAs (a cluster of two) computes tiles of 256 weight rows (the MMA's M, 128 TMEM lanes in each CTA) x 256
+// tokens (its N, 256 TMEM columns) with tcgen05.mma.cta_group::2: each CTA holds its own 128 weight rows and one half
+// of the tokens, so that per SM 32 KB of codes feed 128 x 256 x 256 products.  One CTA alone would have to read 48 KB
+// through the same shared-memory port.  The pairs are persistent and take tiles in a fixed order, tokens first, so
+// that the pairs at work share the weights through L2.
+//
+//   warp 0       one thread: TMA loads of this CTA's codes (128-byte swizzle, stages of 256 columns) and bulk copies
+//                of the scale tiles of its rows and of all 256 tokens
+//   warp 1       leader: one thread copies the stage's scales into both CTAs' tensor memory (tcgen05.cp), issues four
+//                MMAs of 64 columns and the commit that frees the stage in both CTAs; peer: one thread tells the
+//                leader when its stage has landed
+//   warps 2..9   epilogue: 128 of the 256 columns each to registers, tensor memory is free again, then the stores,
+//                while the next tile's MMAs run
+//
+// The accumulators are never split: a chain of K / 64 MMAs truncates, which costs up to 1.2e-7 * K / 512 of the value
+// (measured; nothing while all partial sums are multiples of one unit below 2^24).  Callers with fp32 output whose
+// rows are longer than GEMM_CHAIN_BLOCKS go to the split form (mxfp4_product.cu).
+//
+// Every wait on an mbarrier is bounded; a wait that runs out sets an error bit and an abort flag, all roles fall
+// through to the common exit, outstanding copies are waited for and tensor memory is freed.
+#include <mutex>
+
+#include "axc_kernels.h"
+#include "axc_mx.cuh"
+#include "axc_umma.cuh"
+
+namespace axc {
+namespace {
+
+constexpr uint32_t GM_ROWS = 256, GM_TOKENS = 256;     // tile of a pair
+constexpr uint32_t GM_STAGES = 6;
+constexpr uint32_t GM_W_BYTES = 128 * 128, GM_A_BYTES = 128 * 128;       // codes of a stage in one CTA
+constexpr uint32_t GM_SFW_BYTES = 1024, GM_SFA_BYTES = 2048;
+constexpr uint32_t GM_STAGE_BYTES = GM_W_BYTES + GM_A_BYTES + GM_SFW_BYTES + GM_SFA_BYTES;
+constexpr uint32_t GM_OFF_A = GM_W_BYTES, GM_OFF_SFW = GM_OFF_A + GM_A_BYTES, GM_OFF_SFA = GM_OFF_SFW + GM_SFW_BYTES;
+constexpr uint32_t GM_OFF_BAR = GM_STAGES * GM_STAGE_BYTES;
+constexpr uint32_t GM_SMEM = GM_OFF_BAR + 256 + 1024;                     // + alignment slack
+constexpr uint32_t GM_EPI_WARPS = 8;
+constexpr uint32_t GM_THREADS = (2 + GM_EPI_WARPS) * 32;
+constexpr uint32_t GM_SF_COL = 256;                    // scale columns behind the accumulator: 2 slots of 24
+static_assert(GM_STAGE_BYTES % 1024 == 0, "the swizzled tiles need 1024-byte alignment");
+static_assert(GM_SMEM <= 227 * 1024, "one CTA per SM");
+
+struct GmArgs {
+    const uint8_t* w_scales;
+    const uint8_t* a_scales;
+    void* c;
+    uint32_t m, rows, n_blocks;
+    uint32_t token_tiles, tiles;
+    uint32_t* status;
+};
+
+struct GmBars {
+    uint64_t full[GM_STAGES], empty[GM_STAGES];
+    uint64_t acc_full, acc_empty;
+    uint32_t tmem_base;
+    volatile uint32_t abort;
+};
+
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint32_t smem_addr) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(mx_scale_desc(smem_addr)) : "memory");
+}
+
+__device__ __forceinline__ void umma_mxf4_pair(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
+                                               uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+
+template <typename Out>
+__global__ void __launch_bounds__(GM_THREADS, 1)
+mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const GmArgs p) {
+    extern __shared__ uint8_t smem_dyn[];
+    const uint32_t raw_addr = smem_u32(smem_dyn);
+    const uint32_t base = (raw_addr + 1023u) & ~1023u;
+    uint8_t* sm = smem_dyn + (base - raw_addr);
+    GmBars* bars = reinterpret_cast<GmBars*>(sm + GM_OFF_BAR);
+
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    uint32_t rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const bool leader = rank == 0;
+    const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t n_st = (p.n_blocks + 7u) / 8u, n_quads = (p.n_blocks + 3u) / 4u;
+    const uint32_t row_tiles = (p.rows + 127u) / 128u, tok_tiles = (p.m + 127u) / 128u;   // scale tiles of W and A
+
+    if (tid == 0) {
+        for (uint32_t s = 0; s < GM_STAGES; ++s) mbar_init(&bars->full[s], leader ? 2u : 1u), mbar_init(&bars->empty[s], 1);
+        mbar_init(&bars->acc_full, 1);
+        mbar_init(&bars->acc_empty, leader ? 2u * GM_EPI_WARPS : 1u);
+        bars->abort = 0;
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync_all();   // both CTAs' barriers exist before anyone arrives remotely
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = bars->tmem_base;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // an ordered launch: see axc_tuning.pdl
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t issued = 0;
+            for (uint32_t tile = pair; tile < p.tiles && !bars->abort; tile += pairs) {
+                const uint32_t row0 = tile / p.token_tiles * GM_ROWS + rank * 128u, tok0 = tile % p.token_tiles * GM_TOKENS;
+                // scale tiles that exist: the last pair may have no rows in its second CTA, the last tokens one tile
+                const bool has_rows = row0 / 128u < row_tiles;
+                const uint32_t a_tiles = min(2u, tok_tiles - tok0 / 128u);
+                const uint8_t* sw = p.w_scales + (uint64_t)(row0 / 128u) * n_quads * MX_TILE_BYTES;
+                const uint8_t* sa = p.a_scales + (uint64_t)(tok0 / 128u) * n_quads * MX_TILE_BYTES;
+                for (uint32_t st = 0; st < n_st && !bars->abort; ++st, ++issued) {
+                    const uint32_t s = issued % GM_STAGES, ph = (issued / GM_STAGES) & 1u;
+                    if (!mbar_wait(&bars->empty[s], ph ^ 1u, p.status)) {
+                        bars->abort = 1;
+                        break;
+                    }
+                    const uint32_t quad_bytes = min(2u, n_quads - st * 2u) * MX_TILE_BYTES;
+                    uint8_t* stage = sm + s * GM_STAGE_BYTES;
+                    mbar_expect_tx(&bars->full[s], GM_W_BYTES + GM_A_BYTES + ((has_rows ? 1u : 0u) + a_tiles) * quad_bytes);
+                    tma_load_2d(base + s * GM_STAGE_BYTES, &tm_w, (int32_t)(st * 128u), (int32_t)row0, &bars->full[s]);
+                    tma_load_2d(base + s * GM_STAGE_BYTES + GM_OFF_A, &tm_a, (int32_t)(st * 128u), (int32_t)(tok0 + rank * 128u),
+                                &bars->full[s]);
+                    if (has_rows) bulk_g2s(stage + GM_OFF_SFW, sw + st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
+                    for (uint32_t q = 0; q < a_tiles; ++q)
+                        bulk_g2s(stage + GM_OFF_SFA + q * 1024u, sa + ((uint64_t)q * n_quads + st * 2u) * MX_TILE_BYTES, quad_bytes,
+                                 &bars->full[s]);
+                }
+            }
+            // nothing may still be in flight towards this CTA's shared memory at exit
+            for (uint32_t j = issued > GM_STAGES ? issued - GM_STAGES : 0; j < issued; ++j)
+                (void)mbar_wait(&bars->full[j % GM_STAGES], (j / GM_STAGES) & 1u, p.status);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            bool ok = true;
+            uint32_t it = 0, done = 0;
+            for (uint32_t tile = pair; tile < p.tiles && ok && !bars->abort; tile += pairs, ++done) {
+                ok = mbar_wait(&bars->acc_empty, (done & 1u) ^ 1u, p.status);   // the epilogue has read the last tile
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (uint32_t st = 0; st < n_st && !bars->abort; ++st, ++it) {
+                    const uint32_t s = it % GM_STAGES, ph = (it / GM_STAGES) & 1u;
+                    ok = mbar_wait(&bars->full[s], ph, p.status);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t slot = tmem + GM_SF_COL + (it & 1u) * 24u, stage = base + s * GM_STAGE_BYTES;
+                    const uint32_t steps = min(4u, (p.n_blocks - st * 8u + 1u) / 2u);
+                    for (uint32_t g = 0; g < (steps + 1u) / 2u; ++g) {
+                        scales_to_tmem_pair(slot + g * 4u, stage + GM_OFF_SFW + g * MX_TILE_BYTES);
+                        scales_to_tmem_pair(slot + 8u + g * 8u, stage + GM_OFF_SFA + g * MX_TILE_BYTES);
+                        scales_to_tmem_pair(slot + 12u + g * 8u, stage + GM_OFF_SFA + 1024u + g * MX_TILE_BYTES);
+                    }
+                    const uint64_t wd = sw128_desc(stage), ad = sw128_desc(stage + GM_OFF_A);
+                    for (uint32_t kk = 0; kk < steps; ++kk)
+                        umma_mxf4_pair(tmem, wd + 2u * kk, ad + 2u * kk, mx_idesc(256u, GM_TOKENS, (kk & 1u) * 2u),
+                                       slot + (kk >> 1) * 4u, slot + 8u + (kk >> 1) * 8u, (st | kk) != 0u);
+                    umma_commit_pair(&bars->empty[s]);
+                }
+                if (!ok) break;
+                umma_commit_pair(&bars->acc_full);
+            }
+            if (!ok) bars->abort = 1;
+        } else if (lane == 0) {
+            // peer: tell the leader when this CTA's stage has landed
+            uint32_t it = 0;
+            for (uint32_t tile = pair; tile < p.tiles && !bars->abort; tile += pairs)
+                for (uint32_t st = 0; st < n_st && !bars->abort; ++st, ++it) {
+                    if (!mbar_wait(&bars->full[it % GM_STAGES], (it / GM_STAGES) & 1u, p.status)) {
+                        bars->abort = 1;
+                        break;
+                    }
+                    mbar_arrive_remote(&bars->full[it % GM_STAGES], 0u);
+                }
+        }
+    } else {
+        // ---------------- epilogue: TMEM lane = weight row, column = token ----------------
+        const uint32_t quad = warp & 3u, half = (warp - 2u) >> 2;   // warps 2..5: tokens 0..127, warps 6..9: 128..255
+        uint32_t done = 0;
+        bool ok = true;
+        for (uint32_t tile = pair; tile < p.tiles && ok; tile += pairs, ++done) {
+            const uint32_t row = tile / p.token_tiles * GM_ROWS + rank * 128u + quad * 32u + lane;
+            const uint32_t tok0 = tile % p.token_tiles * GM_TOKENS + half * 128u;
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bars->acc_full, done & 1u, p.status) && !bars->abort);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            uint32_t v[4][32];
+#pragma unroll
+            for (uint32_t b = 0; b < 4u; ++b) tmem_load32(tmem + ((quad * 32u) << 16) + half * 128u + b * 32u, v[b]);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if (leader) mbar_arrive(&bars->acc_empty);
+                else mbar_arrive_remote(&bars->acc_empty, 0u);
+            }
+            if (row < p.rows) {
+                Out* dst = reinterpret_cast<Out*>(p.c) + (uint64_t)tok0 * p.rows + row;
+#pragma unroll
+                for (uint32_t b = 0; b < 4u; ++b)
+#pragma unroll
+                    for (uint32_t j = 0; j < 32u; ++j)
+                        if (tok0 + b * 32u + j < p.m) put(dst + (uint64_t)(b * 32u + j) * p.rows, __uint_as_float(v[b][j]));
+            }
+        }
+        if (!ok) bars->abort = 1;
+    }
+
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync_all();   // no remote arrive or multicast commit may still target a CTA that left
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <typename Out>
+cudaError_t launch(const CUtensorMap& tm_w, const CUtensorMap& tm_a, const GmArgs& p, cudaStream_t stream, int sm_count) {
+    auto kern = mx_gemm_kernel<Out>;
+    cudaLaunchConfig_t cfg{};
+    cfg.blockDim = dim3(GM_THREADS), cfg.dynamicSmemBytes = GM_SMEM, cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    int pairs = sm_count / 2;
+    {   // once per device: raise the shared-memory limit, ask how many pairs fit at once
+        static std::mutex mu;
+        static int fits[64] = {};
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        std::lock_guard<std::mutex> lock(mu);
+        if (dev < 0 || dev >= 64 || fits[dev] == 0) {
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GM_SMEM);
+            if (e != cudaSuccess) return e;
+            int n = 0;
+            cfg.gridDim = dim3(2u * (unsigned)pairs), cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) n = pairs, cudaGetLastError();
+            if (dev >= 0 && dev < 64) fits[dev] = n;
+            if (n < pairs) pairs = n;
+        } else if (fits[dev] < pairs) {
+            pairs = fits[dev];
+        }
+    }
+    cfg.gridDim = dim3(2u * (p.tiles < (uint32_t)pairs ? p.tiles : (uint32_t)pairs)), cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, tm_w, tm_a, p);
+}
+
+}  // namespace
+
+cudaError_t launch_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* a_codes, const uint8_t* a_scales,
+                              void* c, ElemType type, uint32_t m_tokens, uint32_t n_rows, uint32_t n_blocks,
+                              uint32_t* status, cudaStream_t stream, int sm_count) {
+    if (!tensor_map_encoder()) return cudaErrorNotSupported;
+    CUtensorMap tm_w, tm_a;
+    if (!mx_encode_codes(&tm_w, w_codes, n_rows, n_blocks, 128u) || !mx_encode_codes(&tm_a, a_codes, m_tokens, n_blocks, 128u))
+        return cudaErrorInvalidValue;
+    GmArgs p{w_scales, a_scales, c, m_tokens, n_rows, n_blocks, (m_tokens + GM_TOKENS - 1u) / GM_TOKENS, 0, status};
+    p.tiles = (n_rows + GM_ROWS - 1u) / GM_ROWS * p.token_tiles;
+    switch (type) {
+        case ElemType::F32: return launch<float>(tm_w, tm_a, p, stream, sm_count);
+        case ElemType::BF16: return launch<__nv_bfloat16>(tm_w, tm_a, p, stream, sm_count);
+        case ElemType::F16: return launch<__half>(tm_w, tm_a, p, stream, sm_count);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace axc

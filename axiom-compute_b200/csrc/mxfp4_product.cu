@@ -29,9 +29,6 @@
 //
 // Every wait on an mbarrier is bounded; a wait that runs out sets an error bit and an abort flag, all roles fall
 // through to the common exit, outstanding copies are waited for and tensor memory is freed.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
 #include <mutex>
 
 #include "axc_kernels.h"
@@ -47,19 +44,8 @@ constexpr uint32_t MP_CHAIN = 16;                   // stages per accumulator: 4
 constexpr uint32_t MP_MAX_STAGES = 12;
 constexpr uint32_t MP_ROW_WARPS = 4, MP_X_WARPS = 4;
 
-// kind::mxf4 instruction descriptor: both operands E2M1 (1 at bits 7 and 10), K-major, E8M0 scales (bit 23), M = 128
-// (M >> 7 at bit 27), N >> 3 at bit 17; the scale ids (which two of the four bytes of a column) at bits 4 and 29.
-__device__ __forceinline__ uint32_t mx_idesc(uint32_t n, uint32_t sf_id) {
-    return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | (1u << 27) | (sf_id << 4) | (sf_id << 29);
-}
-
-// Shared-memory descriptor of a 512-byte scale tile: 32 rows of 16 bytes, no swizzle, 8 rows 128 bytes apart.
-__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
-    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | (8ull << 16) | (8ull << 32) | (1ull << 46);
-}
-
 __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem_addr) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(scale_desc(smem_addr)) : "memory");
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(mx_scale_desc(smem_addr)) : "memory");
 }
 
 __device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
@@ -223,7 +209,7 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
                 const uint32_t chain = min(st / MP_CHAIN, p.n_acc - 1u);
                 const uint32_t first = st == chain * MP_CHAIN;   // the chain's first stage overwrites its accumulator
                 for (uint32_t kk = 0; kk < steps; ++kk)          // 64 codes = 32 bytes = 2 descriptor units per step
-                    umma_mxf4(tmem + chain * p.n, ad + 2u * kk, bd + 2u * kk, mx_idesc(p.n, (kk & 1u) * 2u),
+                    umma_mxf4(tmem + chain * p.n, ad + 2u * kk, bd + 2u * kk, mx_idesc(128u, p.n, (kk & 1u) * 2u),
                               slot + (kk >> 1) * 4u, slot + 8u + (kk >> 1) * b_tiles * 4u, !(first && kk == 0u));
                 umma_commit(&bars->empty[s]);
             }
@@ -353,17 +339,6 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     }
 }
 
-bool encode_codes(CUtensorMap* map, const uint8_t* codes, uint32_t rows, uint32_t n_blocks, uint32_t box_rows) {
-    auto encode = tensor_map_encoder();
-    cuuint64_t dims[2] = {(uint64_t)n_blocks * MX_BLOCK_BYTES, rows};
-    cuuint64_t strides[1] = {(uint64_t)n_blocks * MX_BLOCK_BYTES};
-    cuuint32_t box[2] = {MP_STAGE_BYTES, box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <bool DIGITS>
 cudaError_t launch(const uint8_t* w_codes, const uint8_t* a_codes, MpArgs p, uint32_t smem_budget, uint32_t token_tiles,
                    cudaStream_t stream) {
@@ -396,9 +371,9 @@ cudaError_t launch(const uint8_t* w_codes, const uint8_t* a_codes, MpArgs p, uin
     p.n_acc = (cols - sf_cols) / p.n;
     if (p.n_acc > want) p.n_acc = want;
     CUtensorMap tm_w, tm_a;
-    if (!encode_codes(&tm_w, w_codes, p.rows, p.n_blocks, p.rows_per_cta)) return cudaErrorInvalidValue;
+    if (!mx_encode_codes(&tm_w, w_codes, p.rows, p.n_blocks, p.rows_per_cta)) return cudaErrorInvalidValue;
     if (DIGITS) tm_a = tm_w;
-    else if (!encode_codes(&tm_a, a_codes, p.m, p.n_blocks, p.n)) return cudaErrorInvalidValue;
+    else if (!mx_encode_codes(&tm_a, a_codes, p.m, p.n_blocks, p.n)) return cudaErrorInvalidValue;
     auto kern = mx_product_kernel<DIGITS>;
     {
         static std::mutex mu;
@@ -444,6 +419,8 @@ cudaError_t launch_mxfp4_prefill(const uint8_t* w_codes, const uint8_t* w_scales
                                  const uint8_t* a_scales, void* c, ElemType type, uint32_t m_tokens, uint32_t n_rows,
                                  uint32_t n_blocks, uint32_t* status, cudaStream_t stream, int sm_count) {
     if (m_tokens == 0 || n_rows == 0 || n_blocks == 0) return cudaSuccess;
+    if (m_tokens > 64u)
+        return launch_mxfp4_gemm(w_codes, w_scales, a_codes, a_scales, c, type, m_tokens, n_rows, n_blocks, status, stream, sm_count);
     MpArgs p{};
     p.w_scales = w_scales, p.a_scales = a_scales, p.out = c, p.m = m_tokens, p.rows = n_rows, p.n_blocks = n_blocks;
     p.status = status, p.out_type = (uint32_t)type;

@@ -74,26 +74,6 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc,
         : "memory");
 }
 
-// Arrives (once the MMAs issued so far have completed) on the barrier at this shared-memory
-// offset in both CTAs of the pair.
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-            smem_u32(bar)),
-        "h"((uint16_t)3)
-        : "memory");
-}
-
-// Arrive on the barrier at the same offset in CTA `cta` of the cluster.
-__device__ __forceinline__ void mbar_arrive_remote(uint64_t* bar, uint32_t cta) {
-    asm volatile(
-        "{\n\t.reg .b32 r;\n\t"
-        "mapa.shared::cluster.u32 r, %0, %1;\n\t"
-        "mbarrier.arrive.shared::cluster.b64 _, [r];\n\t}" ::"r"(smem_u32(bar)),
-        "r"(cta)
-        : "memory");
-}
-
 // Bounded wait that also acquires what other CTAs of the cluster released before arriving.
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* err) {
     const uint32_t addr = smem_u32(bar);
@@ -110,10 +90,6 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
     }
     if (err) atomicOr(err, ERR_BULK_WAIT_TIMEOUT);
     return false;
-}
-
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {

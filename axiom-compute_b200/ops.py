@@ -169,95 +169,111 @@ def _count(value, name: str, least: int = 0) -> int:
     return value
 
 
-def _same_device(first: torch.Tensor, **others) -> None:
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, the first operand on {first.device}")
+def _ptr(t: torch.Tensor, dtype, name: str, min_elems: int, device: int) -> int:
+    """``_chk``, and on CUDA device `device`.  (A small call is bound by the host: the checks that pass are kept to a
+    few attribute reads.)"""
+    if t.dtype is dtype and t.is_cuda and t.is_contiguous() and t.numel() >= min_elems:
+        if t.get_device() != device:
+            raise ValueError(f"{name} is on {t.device}, the first operand on cuda:{device}")
+        return t.data_ptr()
+    return _chk(t, dtype, name, min_elems)      # says what is wrong
 
 
-def _out(t: Optional[torch.Tensor], shape, dtype, device, name: str):
-    """The caller's output tensor after its checks, or a new one."""
-    if t is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    n = 1
-    for d in shape:
-        n *= d
-    _chk(t, dtype, name, n)
-    return t
+def _device_of(t: torch.Tensor, name: str) -> int:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (this backend has no CPU path)")
+    return t.get_device()
 
 
-def _status_ptr(status: Optional[torch.Tensor]):
-    return _chk(status, torch.int32, "status", 1) if status is not None else None
-
-
-def _launch(device: torch.device, fn, *args) -> None:
-    """fn(*args, stream) on `device`'s current stream."""
-    if device.index == torch.cuda.current_device():
-        _raise_for(fn(*args[:-1], int(torch.cuda.current_stream().cuda_stream), *args[-1]))
+def _launch(device: int, fn, *args) -> None:
+    """fn(*args[:-1], stream, *args[-1]) on the current stream of CUDA device `device`."""
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args[:-1], stream, *args[-1])
     else:
         with torch.cuda.device(device):
-            _raise_for(fn(*args[:-1], int(torch.cuda.current_stream().cuda_stream), *args[-1]))
+            rc = fn(*args[:-1], stream, *args[-1])
+    if rc:
+        _raise_for(rc)
+
+
+def _status_ptr(status: Optional[torch.Tensor], device: int):
+    return None if status is None else _ptr(status, torch.int32, "status", 1, device)
 
 
 def mxfp4_scale_bytes(rows: int, n_blocks: int) -> int:
     """Bytes of the scale tiles of an MXFP4 matrix (tiles of 128 rows x 4 blocks)."""
-    return (_count(rows, "rows") + 127) // 128 * ((_count(n_blocks, "n_blocks") + 3) // 4) * 512
+    return _tile_bytes(_count(rows, "rows"), _count(n_blocks, "n_blocks"))
+
+
+def _tile_bytes(rows: int, n_blocks: int) -> int:
+    return (rows + 127) // 128 * ((n_blocks + 3) // 4) * 512
+
+
+def _mx_operand(codes, scales, rows: int, n_blocks: int, name: str, device: int):
+    return (_ptr(codes, torch.uint8, name + "codes", rows * n_blocks * MX_BLOCK_BYTES, device),
+            _ptr(scales, torch.uint8, name + "scales", _tile_bytes(rows, n_blocks), device))
 
 
 def mxfp4_quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None):
     """Rows of a float32, bfloat16 or float16 tensor to MXFP4: returns (codes, scales), uint8 tensors of
     rows x ceil(cols / 32) * 16 bytes and of ``mxfp4_scale_bytes`` (layout: include/axc_cuda.h).  x has shape
     (rows, cols) or (cols,); its last dimension is contiguous, rows may be any stride apart."""
-    if not x.is_cuda:
-        raise ValueError("x must be a CUDA tensor (this backend has no CPU path)")
+    device = _device_of(x, "x")
     xt = _float_type(x.dtype, "x")
-    if x.dim() not in (1, 2):
+    shape, strides = x.shape, x.stride()
+    if len(shape) == 2:
+        rows, cols = shape
+        stride = strides[0] if rows > 1 else cols
+    elif len(shape) == 1:
+        rows, cols = 1, shape[0]
+        stride = cols
+    else:
         raise ValueError(f"x must have one or two dimensions, got {x.dim()}")
-    rows, cols = (1, x.shape[0]) if x.dim() == 1 else (x.shape[0], x.shape[1])
-    if cols > 1 and x.stride(-1) != 1:
+    if cols > 1 and strides[-1] != 1:
         raise ValueError("the last dimension of x must be contiguous")
-    stride = x.stride(0) if x.dim() == 2 and rows > 1 else cols
     if stride < cols:
         raise ValueError("the rows of x overlap")
     _count(rows, "rows"), _count(cols, "cols")
     n_blocks = (cols + 31) // 32
-    codes = _out(codes, (rows, n_blocks * MX_BLOCK_BYTES), torch.uint8, x.device, "codes")
-    scales = _out(scales, (mxfp4_scale_bytes(rows, n_blocks),), torch.uint8, x.device, "scales")
-    _same_device(x, codes=codes, scales=scales)
-    _launch(x.device, _ffi.lib().axc_cuda_mxfp4_quantize, x.data_ptr(), xt, stride, rows, cols, codes.data_ptr(),
-            scales.data_ptr(), ())
+    if codes is None:
+        codes = x.new_empty((rows, n_blocks * MX_BLOCK_BYTES), dtype=torch.uint8)
+    if scales is None:
+        scales = x.new_empty(_tile_bytes(rows, n_blocks), dtype=torch.uint8)
+    cp, sp = _mx_operand(codes, scales, rows, n_blocks, "", device)
+    _launch(device, _ffi.lib().axc_cuda_mxfp4_quantize, x.data_ptr(), xt, stride, rows, cols, cp, sp, ())
     return codes, scales
-
-
-def _mx_operand(codes, scales, rows: int, n_blocks: int, name: str):
-    return (_chk(codes, torch.uint8, f"{name}codes", rows * n_blocks * MX_BLOCK_BYTES),
-            _chk(scales, torch.uint8, f"{name}scales", mxfp4_scale_bytes(rows, n_blocks)))
 
 
 def mxfp4_dequant(codes: torch.Tensor, scales: torch.Tensor, rows: int, n_blocks: int,
                   out_dtype: torch.dtype = torch.float32, w: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values of an MXFP4 matrix, shape (rows, n_blocks * 32): exact in float32, rounded to nearest even in
     bfloat16 / float16."""
+    device = _device_of(codes, "codes")
     rows, n_blocks = _count(rows, "rows"), _count(n_blocks, "n_blocks")
-    cp, sp = _mx_operand(codes, scales, rows, n_blocks, "")
+    cp, sp = _mx_operand(codes, scales, rows, n_blocks, "", device)
     wt = _float_type(out_dtype, "out_dtype")
-    w = _out(w, (rows, n_blocks * MX_BLOCK_ELEMS), out_dtype, codes.device, "w")
-    _same_device(codes, scales=scales, w=w)
-    _launch(codes.device, _ffi.lib().axc_cuda_mxfp4_dequant, cp, sp, w.data_ptr(), wt, rows, n_blocks, ())
+    if w is None:
+        w = codes.new_empty((rows, n_blocks * MX_BLOCK_ELEMS), dtype=out_dtype)
+    wp = _ptr(w, out_dtype, "w", rows * n_blocks * MX_BLOCK_ELEMS, device)
+    _launch(device, _ffi.lib().axc_cuda_mxfp4_dequant, cp, sp, wp, wt, rows, n_blocks, ())
     return w
 
 
 def mxfp4_matvec(codes: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, rows: int, n_blocks: int,
                  y: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None, m_tokens: int = 1) -> torch.Tensor:
     """y[t, r] = sum_k W[r, k] x[t, k] with W in MXFP4, for 1 to 8 float32 vectors x of n_blocks * 32 values; x keeps
-    its precision (include/axc_cuda.h).  y has shape (rows,) for one token, else (m_tokens, rows)."""
+    its precision (include/axc_cuda.h).  y has shape (rows,) for one vector, (m_tokens, rows) where x has more
+    dimensions than one or there are several."""
+    device = _device_of(codes, "codes")
     rows, n_blocks, m_tokens = _count(rows, "rows"), _count(n_blocks, "n_blocks"), _count(m_tokens, "m_tokens", 1)
-    cp, sp = _mx_operand(codes, scales, rows, n_blocks, "")
-    xp = _chk(x, torch.float32, "x", m_tokens * n_blocks * MX_BLOCK_ELEMS)
-    y = _out(y, (m_tokens, rows) if x.dim() > 1 or m_tokens > 1 else (rows,), torch.float32, codes.device, "y")
-    _same_device(codes, scales=scales, x=x, y=y, status=status)
-    _launch(codes.device, _ffi.lib().axc_cuda_mxfp4_matvec, cp, sp, xp, y.data_ptr(), m_tokens, rows, n_blocks,
-            (_status_ptr(status),))
+    cp, sp = _mx_operand(codes, scales, rows, n_blocks, "", device)
+    xp = _ptr(x, torch.float32, "x", m_tokens * n_blocks * MX_BLOCK_ELEMS, device)
+    if y is None:
+        y = x.new_empty((m_tokens, rows) if m_tokens > 1 or x.dim() > 1 else rows)
+    yp = _ptr(y, torch.float32, "y", m_tokens * rows, device)
+    _launch(device, _ffi.lib().axc_cuda_mxfp4_matvec, cp, sp, xp, yp, m_tokens, rows, n_blocks,
+            (_status_ptr(status, device),))
     return y
 
 
@@ -266,26 +282,30 @@ def mxfp4_prefill(w_codes: torch.Tensor, w_scales: torch.Tensor, a_codes: torch.
                   status: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """C[m, n] = sum_k A[m, k] W[n, k] on the tensor cores, both operands in MXFP4 (tokens through
     ``mxfp4_quantize``): C has shape (m_tokens, n_rows) in out_dtype, fp32 accumulation, one rounding."""
+    device = _device_of(w_codes, "w_codes")
     m_tokens, n_rows, n_blocks = _count(m_tokens, "m_tokens"), _count(n_rows, "n_rows"), _count(n_blocks, "n_blocks")
-    wp, wsp = _mx_operand(w_codes, w_scales, n_rows, n_blocks, "w_")
-    ap, asp = _mx_operand(a_codes, a_scales, m_tokens, n_blocks, "a_")
+    wp, wsp = _mx_operand(w_codes, w_scales, n_rows, n_blocks, "w_", device)
+    ap, asp = _mx_operand(a_codes, a_scales, m_tokens, n_blocks, "a_", device)
     ct = _float_type(out_dtype, "out_dtype")
-    c = _out(c, (m_tokens, n_rows), out_dtype, w_codes.device, "c")
-    _same_device(w_codes, w_scales=w_scales, a_codes=a_codes, a_scales=a_scales, c=c, status=status)
-    _launch(w_codes.device, _ffi.lib().axc_cuda_mxfp4_prefill, wp, wsp, ap, asp, c.data_ptr(), ct, m_tokens, n_rows, n_blocks,
-            (_status_ptr(status),))
+    if c is None:
+        c = w_codes.new_empty((m_tokens, n_rows), dtype=out_dtype)
+    cp = _ptr(c, out_dtype, "c", m_tokens * n_rows, device)
+    _launch(device, _ffi.lib().axc_cuda_mxfp4_prefill, wp, wsp, ap, asp, cp, ct, m_tokens, n_rows, n_blocks,
+            (_status_ptr(status, device),))
     return c
 
 
-def _embed(fn, ptrs, first: torch.Tensor, ids, rows: int, n: int, elems: int, scale, out, out_dtype, status, others):
-    if not ids.is_cuda or ids.dtype not in _ID_TYPES or not ids.is_contiguous():
+def _embed(fn, ptrs, device: int, ids, rows: int, n: int, elems: int, scale, out, out_dtype, status):
+    it = _ID_TYPES.get(ids.dtype)
+    if it is None or not ids.is_cuda or not ids.is_contiguous():
         raise ValueError("ids must be a contiguous int32 or int64 CUDA tensor")
     n_ids = _count(ids.numel(), "the number of ids")
     ot = _float_type(out_dtype, "out_dtype")
-    out = _out(out, tuple(ids.shape) + (n * elems,), out_dtype, first.device, "out")
-    _same_device(first, ids=ids, out=out, status=status, **others)
-    _launch(first.device, fn, *ptrs, ids.data_ptr(), _ID_TYPES[ids.dtype], n_ids, out.data_ptr(), ot, rows, n, float(scale),
-            (_status_ptr(status),))
+    ip = _ptr(ids, ids.dtype, "ids", 0, device)
+    if out is None:
+        out = ids.new_empty((*ids.shape, n * elems), dtype=out_dtype)
+    op = _ptr(out, out_dtype, "out", n_ids * n * elems, device)
+    _launch(device, fn, *ptrs, ip, it, n_ids, op, ot, rows, n, scale, (_status_ptr(status, device),))
     return out
 
 
@@ -294,24 +314,27 @@ def q4k_embed(q: torch.Tensor, ids: torch.Tensor, rows: int, n_superblocks: int,
               status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[..., :] = dequant(row ids[...] of a Q4_K_M matrix) * scale, rounded once to out_dtype.  An id outside
     [0, rows) gives a row of zeros and sets bit 1 (value 2) of status."""
+    device = _device_of(q, "q")
     rows, n = _count(rows, "rows"), _count(n_superblocks, "n_superblocks")
-    qp = _chk(q, torch.uint8, "q", rows * n * Q4K_SB_BYTES)
-    return _embed(_ffi.lib().axc_cuda_q4k_embed, (qp,), q, ids, rows, n, Q4K_SB_ELEMS, scale, out, out_dtype, status, {})
+    qp = _ptr(q, torch.uint8, "q", rows * n * Q4K_SB_BYTES, device)
+    return _embed(_ffi.lib().axc_cuda_q4k_embed, (qp,), device, ids, rows, n, Q4K_SB_ELEMS, scale, out, out_dtype, status)
 
 
 def q4_0_embed(q: torch.Tensor, ids: torch.Tensor, rows: int, n_blocks: int, scale: float = 1.0,
                out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
                status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``q4k_embed`` for a Q4_0 matrix."""
+    device = _device_of(q, "q")
     rows, n = _count(rows, "rows"), _count(n_blocks, "n_blocks")
-    qp = _chk(q, torch.uint8, "q", rows * n * Q4_0_BLK_BYTES)
-    return _embed(_ffi.lib().axc_cuda_q4_0_embed, (qp,), q, ids, rows, n, Q4_0_BLK_ELEMS, scale, out, out_dtype, status, {})
+    qp = _ptr(q, torch.uint8, "q", rows * n * Q4_0_BLK_BYTES, device)
+    return _embed(_ffi.lib().axc_cuda_q4_0_embed, (qp,), device, ids, rows, n, Q4_0_BLK_ELEMS, scale, out, out_dtype, status)
 
 
 def mxfp4_embed(codes: torch.Tensor, scales: torch.Tensor, ids: torch.Tensor, rows: int, n_blocks: int, scale: float = 1.0,
                 out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
                 status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``q4k_embed`` for an MXFP4 matrix."""
+    device = _device_of(codes, "codes")
     rows, n = _count(rows, "rows"), _count(n_blocks, "n_blocks")
-    return _embed(_ffi.lib().axc_cuda_mxfp4_embed, _mx_operand(codes, scales, rows, n, ""), codes, ids, rows, n, MX_BLOCK_ELEMS,
-                  scale, out, out_dtype, status, {"scales": scales})
+    return _embed(_ffi.lib().axc_cuda_mxfp4_embed, _mx_operand(codes, scales, rows, n, "", device), device, ids, rows, n,
+                  MX_BLOCK_ELEMS, scale, out, out_dtype, status)
