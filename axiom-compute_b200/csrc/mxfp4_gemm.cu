@@ -112,7 +112,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
     __syncthreads();
     cluster_sync_all();   // both CTAs' barriers exist before anyone arrives remotely
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = bars->tmem_base;
+    const uint32_t tmem = bars->tmem_base;   // 0: all columns are this CTA's (the MMA loop counts on it)
     asm volatile("griddepcontrol.wait;" ::: "memory");   // an ordered launch: see axc_tuning.pdl
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -149,35 +149,43 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
                 (void)mbar_wait(&bars->full[j % GM_STAGES], (j / GM_STAGES) & 1u, p.status);
         }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
+        if (leader) {
+            // The whole warp runs the loop, an elected lane issues.
             bool ok = true;
-            uint32_t it = 0, done = 0;
-            for (uint32_t tile = pair; tile < p.tiles && ok && !bars->abort; tile += pairs, ++done) {
-                ok = mbar_wait(&bars->acc_empty, (done & 1u) ^ 1u, p.status);   // the epilogue has read the last tile
+            uint32_t s = 0, ph = 0, slot = 0, acc_ph = 1;
+            for (uint32_t tile = pair; tile < p.tiles && ok; tile += pairs, acc_ph ^= 1u) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->acc_empty, acc_ph, &bars->abort, p.status));   // the last tile is read
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (uint32_t st = 0; st < n_st && !bars->abort; ++st, ++it) {
-                    const uint32_t s = it % GM_STAGES, ph = (it / GM_STAGES) & 1u;
-                    ok = mbar_wait(&bars->full[s], ph, p.status);
+                for (uint32_t st = 0; st < n_st; ++st) {
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->full[s], ph, &bars->abort, p.status));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t slot = tmem + GM_SF_COL + (it & 1u) * 24u, stage = base + s * GM_STAGE_BYTES;
                     const uint32_t steps = min(4u, (p.n_blocks - st * 8u + 1u) / 2u);
-                    for (uint32_t g = 0; g < (steps + 1u) / 2u; ++g) {
-                        scales_to_tmem_pair(slot + g * 4u, stage + GM_OFF_SFW + g * MX_TILE_BYTES);
-                        scales_to_tmem_pair(slot + 8u + g * 8u, stage + GM_OFF_SFA + g * MX_TILE_BYTES);
-                        scales_to_tmem_pair(slot + 12u + g * 8u, stage + GM_OFF_SFA + 1024u + g * MX_TILE_BYTES);
+                    if (elect_one()) {
+                        const uint32_t sf = GM_SF_COL + slot * 24u, stage = base + s * GM_STAGE_BYTES;
+#pragma unroll
+                        for (uint32_t g = 0; g < 2u; ++g) {
+                            if (2u * g >= steps) break;
+                            scales_to_tmem_pair(sf + g * 4u, stage + GM_OFF_SFW + g * MX_TILE_BYTES);
+                            scales_to_tmem_pair(sf + 8u + g * 8u, stage + GM_OFF_SFA + g * MX_TILE_BYTES);
+                            scales_to_tmem_pair(sf + 12u + g * 8u, stage + GM_OFF_SFA + 1024u + g * MX_TILE_BYTES);
+                        }
+                        const uint64_t wd = sw128_desc(stage), ad = sw128_desc(stage + GM_OFF_A);
+#pragma unroll
+                        for (uint32_t kk = 0; kk < 4u; ++kk) {
+                            if (kk >= steps) break;
+                            umma_mxf4_pair(0u, wd + 2u * kk, ad + 2u * kk, mx_idesc(256u, GM_TOKENS, (kk & 1u) * 2u),
+                                           sf + (kk >> 1) * 4u, sf + 8u + (kk >> 1) * 8u, (st | kk) != 0u);
+                        }
+                        umma_commit_pair(&bars->empty[s]);
+                        if (st + 1u == n_st) umma_commit_pair(&bars->acc_full);
                     }
-                    const uint64_t wd = sw128_desc(stage), ad = sw128_desc(stage + GM_OFF_A);
-                    for (uint32_t kk = 0; kk < steps; ++kk)
-                        umma_mxf4_pair(tmem, wd + 2u * kk, ad + 2u * kk, mx_idesc(256u, GM_TOKENS, (kk & 1u) * 2u),
-                                       slot + (kk >> 1) * 4u, slot + 8u + (kk >> 1) * 8u, (st | kk) != 0u);
-                    umma_commit_pair(&bars->empty[s]);
+                    __syncwarp();
+                    slot ^= 1u;
+                    if (++s == GM_STAGES) s = 0, ph ^= 1u;
                 }
-                if (!ok) break;
-                umma_commit_pair(&bars->acc_full);
             }
-            if (!ok) bars->abort = 1;
         } else if (lane == 0) {
             // peer: tell the leader when this CTA's stage has landed
             uint32_t it = 0;
