@@ -117,21 +117,20 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t issued = 0;
-            for (uint32_t tile = pair; tile < p.tiles && !bars->abort; tile += pairs) {
-                const uint32_t row0 = tile / p.token_tiles * GM_ROWS + rank * 128u, tok0 = tile % p.token_tiles * GM_TOKENS;
-                // scale tiles that exist: the last pair may have no rows in its second CTA, the last tokens one tile
-                const bool has_rows = row0 / 128u < row_tiles;
-                const uint32_t a_tiles = min(2u, tok_tiles - tok0 / 128u);
-                const uint8_t* sw = p.w_scales + (uint64_t)(row0 / 128u) * n_quads * MX_TILE_BYTES;
-                const uint8_t* sa = p.a_scales + (uint64_t)(tok0 / 128u) * n_quads * MX_TILE_BYTES;
-                for (uint32_t st = 0; st < n_st && !bars->abort; ++st, ++issued) {
-                    const uint32_t s = issued % GM_STAGES, ph = (issued / GM_STAGES) & 1u;
-                    if (!mbar_wait(&bars->empty[s], ph ^ 1u, p.status)) {
-                        bars->abort = 1;
-                        break;
-                    }
+        // The whole warp runs the loop, an elected lane issues.
+        uint32_t issued = 0, s = 0, ph = 1;
+        bool ok = true;
+        for (uint32_t tile = pair; tile < p.tiles && ok; tile += pairs) {
+            const uint32_t row0 = tile / p.token_tiles * GM_ROWS + rank * 128u, tok0 = tile % p.token_tiles * GM_TOKENS;
+            // scale tiles that exist: the last pair may have no rows in its second CTA, the last tokens one tile
+            const bool has_rows = row0 / 128u < row_tiles;
+            const uint32_t a_tiles = min(2u, tok_tiles - tok0 / 128u);
+            const uint8_t* sw = p.w_scales + (uint64_t)(row0 / 128u) * n_quads * MX_TILE_BYTES;
+            const uint8_t* sa = p.a_scales + (uint64_t)(tok0 / 128u) * n_quads * MX_TILE_BYTES;
+            for (uint32_t st = 0; st < n_st; ++st, ++issued) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->empty[s], ph, &bars->abort, p.status));
+                if (!ok) break;
+                if (elect_one()) {
                     const uint32_t quad_bytes = min(2u, n_quads - st * 2u) * MX_TILE_BYTES;
                     uint8_t* stage = sm + s * GM_STAGE_BYTES;
                     mbar_expect_tx(&bars->full[s], GM_W_BYTES + GM_A_BYTES + ((has_rows ? 1u : 0u) + a_tiles) * quad_bytes);
@@ -139,15 +138,18 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
                     tma_load_2d(base + s * GM_STAGE_BYTES + GM_OFF_A, &tm_a, (int32_t)(st * 128u), (int32_t)(tok0 + rank * 128u),
                                 &bars->full[s]);
                     if (has_rows) bulk_g2s(stage + GM_OFF_SFW, sw + st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
-                    for (uint32_t q = 0; q < a_tiles; ++q)
-                        bulk_g2s(stage + GM_OFF_SFA + q * 1024u, sa + ((uint64_t)q * n_quads + st * 2u) * MX_TILE_BYTES, quad_bytes,
+                    bulk_g2s(stage + GM_OFF_SFA, sa + st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
+                    if (a_tiles > 1u)
+                        bulk_g2s(stage + GM_OFF_SFA + 1024u, sa + ((uint64_t)n_quads + st * 2u) * MX_TILE_BYTES, quad_bytes,
                                  &bars->full[s]);
                 }
+                __syncwarp();
+                if (++s == GM_STAGES) s = 0, ph ^= 1u;
             }
-            // nothing may still be in flight towards this CTA's shared memory at exit
-            for (uint32_t j = issued > GM_STAGES ? issued - GM_STAGES : 0; j < issued; ++j)
-                (void)mbar_wait(&bars->full[j % GM_STAGES], (j / GM_STAGES) & 1u, p.status);
         }
+        // nothing may still be in flight towards this CTA's shared memory at exit
+        for (uint32_t j = issued > GM_STAGES ? issued - GM_STAGES : 0; j < issued; ++j)
+            (void)mbar_wait(&bars->full[j % GM_STAGES], (j / GM_STAGES) & 1u, p.status);
     } else if (warp == 1) {
         if (leader) {
             // The whole warp runs the loop, an elected lane issues.
