@@ -40,6 +40,11 @@ __device__ __forceinline__ float2 mx_code_pair(uint32_t byte) {
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// One output value, rounded to nearest even.
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+
 // Eight consecutive output values, rounded to nearest even, in one or two 16-byte stores.
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);

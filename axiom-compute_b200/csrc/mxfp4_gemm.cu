@@ -40,8 +40,9 @@ constexpr uint32_t GM_OFF_BAR = GM_STAGES * GM_STAGE_BYTES;
 constexpr uint32_t GM_SMEM = GM_OFF_BAR + 256 + 1024;                     // + alignment slack
 constexpr uint32_t GM_EPI_WARPS = 8;
 constexpr uint32_t GM_THREADS = (2 + GM_EPI_WARPS) * 32;
-constexpr uint32_t GM_SF_COL = 256;                    // scale columns behind the accumulator: 2 slots of 24
+constexpr uint32_t GM_SF_COL = 256;                    // scale columns behind the accumulator: 24 for each stage
 static_assert(GM_STAGE_BYTES % 1024 == 0, "the swizzled tiles need 1024-byte alignment");
+static_assert(GM_SF_COL + GM_STAGES * 24 <= 512, "tensor memory");
 static_assert(GM_SMEM <= 227 * 1024, "one CTA per SM");
 
 struct GmArgs {
@@ -73,10 +74,6 @@ __device__ __forceinline__ void umma_mxf4_pair(uint32_t d, uint64_t a_desc, uint
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
         : "memory");
 }
-
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 
 template <typename Out>
 __global__ void __launch_bounds__(GM_THREADS, 1)
@@ -152,20 +149,19 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
             (void)mbar_wait(&bars->full[j % GM_STAGES], (j / GM_STAGES) & 1u, p.status);
     } else if (warp == 1) {
         if (leader) {
-            // The whole warp runs the loop, an elected lane issues.
             bool ok = true;
-            uint32_t s = 0, ph = 0, slot = 0, acc_ph = 1;
-            for (uint32_t tile = pair; tile < p.tiles && ok; tile += pairs, acc_ph ^= 1u) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->acc_empty, acc_ph, &bars->abort, p.status));   // the last tile is read
+            uint32_t s = 0, ph = 0, acc_ph = 1;
+            if (elect_one()) for (uint32_t tile = pair; tile < p.tiles && ok; tile += pairs, acc_ph ^= 1u) {
+                ok = mbar_wait_or_abort(&bars->acc_empty, acc_ph, &bars->abort, p.status);   // the last tile is read
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (uint32_t st = 0; st < n_st; ++st) {
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->full[s], ph, &bars->abort, p.status));
+                    ok = mbar_wait_or_abort(&bars->full[s], ph, &bars->abort, p.status);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t steps = min(4u, (p.n_blocks - st * 8u + 1u) / 2u);
-                    if (elect_one()) {
-                        const uint32_t sf = GM_SF_COL + slot * 24u, stage = base + s * GM_STAGE_BYTES;
+                    {
+                        const uint32_t sf = GM_SF_COL + s * 24u, stage = base + s * GM_STAGE_BYTES;
 #pragma unroll
                         for (uint32_t g = 0; g < 2u; ++g) {
                             if (2u * g >= steps) break;
@@ -183,8 +179,6 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
                         umma_commit_pair(&bars->empty[s]);
                         if (st + 1u == n_st) umma_commit_pair(&bars->acc_full);
                     }
-                    __syncwarp();
-                    slot ^= 1u;
                     if (++s == GM_STAGES) s = 0, ph ^= 1u;
                 }
             }

@@ -10,22 +10,28 @@
 //             that differ in their scales by factors of 8, and the product with these rows is the same tensor-core
 //             product.  y is the sum of its eight columns.  A weight never passes through a register.
 //
-// A CTA owns up to 128 weight rows (the MMA's M, one TMEM lane each) and one token tile of up to 256 columns (the
-// MMA's N), and streams K through a ring of stages of 256 columns:
+// Both are bound by reading W.  A cluster of `splits` CTAs (1, 2, 4 or 8) owns one or two tiles of 128 weight rows (the
+// MMA's M, one TMEM lane each) and all tokens (its N columns); each CTA takes its share of K, so that small matrices
+// too are spread over the SMs and a CTA has most of its share requested from memory at once.  Stages of 256 columns:
 //
-//   warp 0       one thread: TMA loads of the codes of W (and of A), bulk copies of A's scales
-//   warp 1       one thread: scales from shared into tensor memory (tcgen05.cp), four MMAs of 64 columns per stage,
-//                and the commit that frees the stage; the whole warp allocates and frees tensor memory
-//   warps 2..5   the scales of this CTA's rows, arranged as the MMA takes them; then the epilogue
-//   warps 6..9   matvec only: digits and scales of x
+//   warp 0       TMA loads of the codes of W (and of A), bulk copies of the scale tiles
+//   warps 1, 2   stages in turn: scales from shared into tensor memory (tcgen05.cp), four MMAs of 64 columns per tile and
+//                stage, and the commit that frees the stage.  With few columns an MMA is quick (32 cycles for its 4 KB of
+//                codes) and the issuing thread is the limit, about 550 cycles per stage: two take turns, each with an
+//                accumulator of its own (14336 x 4096, one token: 8.2 -> 7.8 us; four are no faster than two)
+//   warps 3..10  matvec: digits and scales of x, a warp taking 256 columns of one token at a time; then, in both, the
+//                epilogue: every CTA holds partial sums of all its cluster's rows, sends those of each 1/splits of the
+//                rows to the CTA that finishes them (distributed shared memory), and adds what it got in rank order,
+//                so results do not depend on timing.
 //
-// The rows of a CTA need not start at a multiple of 128, so that a matrix spreads over all SMs evenly; that is why
-// warps 2..5 arrange the scales instead of a copy of whole tiles.
+// Each place of the ring has its scale columns in tensor memory, which are free again when the place is.  The
+// accumulators truncate: measured, up to 1.2e-7 of the value per 8 MMAs of a chain when the scales of a row are far apart
+// (and nothing while all partial sums are multiples of one unit below 2^24); a chain is half of a CTA's share of K, and
+// the parts are added in fp32.
 //
-// The accumulators truncate: measured, a chain of K / 64 MMAs loses up to 1.2e-7 * K / 512 of its value when the
-// scales of a row are far apart (and nothing while all partial sums are multiples of one unit below 2^24).  So a
-// chain ends after 4096 columns; the next ones go to further accumulators as long as tensor memory has columns, and
-// the parts are added in fp32 in the epilogue.
+// Tensor memory and clusters: a CTA that waits for its cluster while another of the cluster waits for tensor memory
+// could wait for good, so a CTA's shared memory is at least its share of tensor memory (columns / 512 of an SM), and
+// whatever fits an SM finds its columns.
 //
 // Every wait on an mbarrier is bounded; a wait that runs out sets an error bit and an abort flag, all roles fall
 // through to the common exit, outstanding copies are waited for and tensor memory is freed.
@@ -33,16 +39,19 @@
 
 #include "axc_kernels.h"
 #include "axc_mx.cuh"
-#include "axc_umma.cuh"
 
 namespace axc {
 namespace {
 
 constexpr uint32_t MP_ROWS = 128;
 constexpr uint32_t MP_STAGE_BYTES = 128;            // one stage: 256 columns = 128 bytes of codes per row
-constexpr uint32_t MP_CHAIN = 16;                   // stages per accumulator: 4096 columns
-constexpr uint32_t MP_MAX_STAGES = 12;
-constexpr uint32_t MP_ROW_WARPS = 4, MP_X_WARPS = 4;
+constexpr uint32_t MP_W_BYTES = MP_ROWS * MP_STAGE_BYTES;
+constexpr uint32_t MP_MAX_STAGES = 8;
+constexpr uint32_t MP_PREFETCH = 16;                // stages requested into L2 before the dependency wait
+constexpr uint32_t MP_MMA_WARPS = 2, MP_X_WARPS = 8;
+constexpr uint32_t MP_FIRST_X = 1 + MP_MMA_WARPS;   // warp
+constexpr uint32_t MP_THREADS = (MP_FIRST_X + MP_X_WARPS) * 32;
+constexpr uint32_t MP_SMEM_SM = 228u * 1024u, MP_SMEM_MAX = 227u * 1024u;   // of an SM, of a CTA
 
 __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem_addr) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(mx_scale_desc(smem_addr)) : "memory");
@@ -58,18 +67,25 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a_desc, uint64_t 
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_load8(uint32_t taddr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
 struct MpArgs {
     const uint8_t* w_scales;
     const uint8_t* a_scales;    // prefill
     const float* x;             // matvec
     void* out;
     uint32_t m, rows, n_blocks;
-    uint32_t rows_per_cta;      // 1..128
-    uint32_t n;                 // columns of the MMA = rows of the B operand per token tile
-    uint32_t n_acc, tmem_cols;
+    uint32_t splits, per_shift; // CTAs of a cluster; each finishes 1 << per_shift of its rows
+    uint32_t n;                 // columns of the MMA = rows of the B operand
+    uint32_t tmem_cols;
     uint32_t stages;
-    uint32_t off_b, off_sfa, off_sfb, off_bar, a_stage, b_stage, sfb_stage;   // shared-memory layout
-    uint32_t out_type;
+    uint32_t takers;            // matvec: warps that split x
+    uint32_t off_b, off_sfw, off_sfb, off_red, off_bar;   // shared-memory layout
     uint32_t* status;
 };
 
@@ -80,18 +96,18 @@ struct MpBars {
     volatile uint32_t abort;
 };
 
-// A word of eight octal digits v = -4..3, each as its low three bits in a nibble, to the eight E2M1 codes of v / 2:
-// t = 0..3 is its own code, t = 4..7 stands for t - 8, code 8 | (8 - t) = 16 - t.
-__device__ __forceinline__ uint32_t digit_codes(uint32_t t) {
-    const uint32_t neg = (t >> 2) & 0x11111111u;
-    return (t ^ (neg * 15u)) + neg;
+// Eight octal fields f = v + 4 (v = -4..3), one per nibble, to the eight E2M1 codes of v / 2: v >= 0 is its own code,
+// v < 0 has code 8 | -v = 16 - (v & 7).
+__device__ __forceinline__ uint32_t digit_codes(uint32_t f) {
+    const uint32_t neg = (~f >> 2) & 0x11111111u;
+    return (f ^ 0x44444444u ^ (neg * 15u)) + neg;
 }
 
-// 24 bits = eight octal fields to eight nibbles.
+// 24 bits = eight octal fields to eight nibbles: the upper half of each part moves up (hi * 2^k = hi + hi * (2^k - 1)).
 __device__ __forceinline__ uint32_t spread_octal(uint32_t y) {
-    y = (y & 0xFFFu) | ((y & 0xFFF000u) << 4);
-    y = (y & 0x003F003Fu) | ((y & 0x0FC00FC0u) << 2);
-    return (y & 0x07070707u) | ((y & 0x38383838u) << 1);
+    y += (y & 0x00FFF000u) * 15u;
+    y += (y & 0x0FC00FC0u) * 3u;
+    return y + (y & 0x38383838u);
 }
 
 // 8 x 8 nibbles: w[e] holds digit d of element e in nibble d; afterwards w[d] holds it in nibble e.
@@ -99,7 +115,7 @@ __device__ __forceinline__ void transpose_nibbles(uint32_t (&w)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const uint32_t a = w[i], b = w[i + 1];
-        w[i] = (a & 0x0F0F0F0Fu) | ((b & 0x0F0F0F0Fu) << 4);
+        w[i] = (a & 0x0F0F0F0Fu) | ((b << 4) & 0xF0F0F0F0u);
         w[i + 1] = ((a >> 4) & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u);
     }
 #pragma unroll
@@ -118,15 +134,68 @@ __device__ __forceinline__ void transpose_nibbles(uint32_t (&w)[8]) {
     }
 }
 
-__device__ __forceinline__ void store_out(const MpArgs& p, uint64_t at, float v) {
-    if (p.out_type == (uint32_t)ElemType::F32) reinterpret_cast<float*>(p.out)[at] = v;
-    else if (p.out_type == (uint32_t)ElemType::BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-    else reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(v);
+// max(a, |b|); a NaN stays.
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
 }
 
+__device__ __forceinline__ void load_x(const MpArgs& p, uint32_t st, uint32_t t, uint32_t lane, float (&v)[8]) {
+    const uint32_t k_total = p.n_blocks * 32u, col = st * 256u + lane * 8u;
+    if (col < k_total) {     // k_total is a multiple of 32
+        const float4* src = reinterpret_cast<const float4*>(p.x + (uint64_t)t * k_total + col);
+        const float4 a = __ldg(src), b = __ldg(src + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    }
+}
+
+// Digit codes w[d] of a lane's eight values, and the scale bytes of digit 0 of the four blocks of its half warp with the
+// blocks that hold a value too large to count as finite.
+__device__ __forceinline__ void split_x(const float (&v)[8], uint32_t lane, uint32_t (&w)[8], uint32_t& unit_bytes, uint32_t& nan) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max_abs(most, v[i]);
+    uint32_t top = (uint32_t)__float_as_int(most);
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    // X = rn(x * 2^(22 - e)), e = exponent of the block's largest |x| plus one, so |X| <= 2^22; the unit of digit 0,
+    // with the half that a code counts, is 2^(e - 21): scale byte e - 21 + 127.  Blocks below 2^-104 keep the unit
+    // 2^-126; 2^127 and above count as infinite (scale byte 255, any digits).
+    const uint32_t ex = top >> 23;                                // e = ex - 126
+    const bool bad = ex >= 254u;
+    const uint32_t unit = bad ? 1u : ex > 21u ? ex - 20u : 1u;    // scale byte of digit 0
+    const float factor = __int_as_float((int)((255u - unit) << 23));   // 2^(22 - e) = 2^(128 - unit)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // + 1.5 * 2^23 rounds to an integer in the low mantissa bits; + 4 in every octal digit gives the fields v + 4
+        const float shifted = __fmaf_rn(v[i], factor, 12582912.0f);
+        w[i] = spread_octal((uint32_t)__float_as_int(shifted) + (0x00924924u - 0x4B400000u));
+    }
+    transpose_nibbles(w);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) w[d] = digit_codes(w[d]);
+    const uint32_t at = 8u * ((lane >> 2) & 3u);
+    unit_bytes = unit << at, nan = bad ? 255u << at : 0u;
+    unit_bytes |= __shfl_xor_sync(0xFFFFFFFFu, unit_bytes, 4), nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, 4);
+    unit_bytes |= __shfl_xor_sync(0xFFFFFFFFu, unit_bytes, 8), nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, 8);
+}
+
+// Floats of a row of what one CTA of a cluster sends another: a value per token, or a whole number of groups of eight
+// with four to spare, which spreads the 16-byte accesses of neighbouring rows over the banks.
 template <bool DIGITS>
-__global__ void __launch_bounds__((2 + MP_ROW_WARPS + (DIGITS ? MP_X_WARPS : 0)) * 32, 1)
+__host__ __device__ __forceinline__ uint32_t red_row(uint32_t m) {
+    return DIGITS ? m : (m + 7u) / 8u * 8u + 4u;
+}
+
+template <bool DIGITS, uint32_t TILES, typename Out>
+__global__ void __launch_bounds__(MP_THREADS, 1)
 mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const MpArgs p) {
+    constexpr uint32_t W_STAGE = TILES * MP_W_BYTES, SFW_STAGE = TILES * 1024u, SFB_STAGE = 1024u;
+    constexpr uint32_t SF_COLS = 8u * TILES + 8u;                  // scale columns of a place: B, then the tiles of W
     extern __shared__ uint8_t smem_dyn[];
     const uint32_t raw_addr = smem_u32(smem_dyn);
     const uint32_t base = (raw_addr + 1023u) & ~1023u;   // the swizzled tiles need 1024-byte alignment
@@ -134,16 +203,17 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     MpBars* bars = reinterpret_cast<MpBars*>(sm + p.off_bar);
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-    const uint32_t row0 = blockIdx.x * p.rows_per_cta;
-    const uint32_t tok0 = blockIdx.y * 256u;
-    const uint32_t n_st = (p.n_blocks + 7u) / 8u, n_quads = (p.n_blocks + 3u) / 4u;
-    const uint32_t b_tiles = (p.n + 127u) / 128u;
-    const uint32_t a_tiles = DIGITS ? 0u : min(b_tiles, (p.m - tok0 + 127u) / 128u);   // scale tiles that A has here
+    const uint32_t group = blockIdx.x / p.splits, rank = blockIdx.x - group * p.splits;
+    const uint32_t tile0 = group * TILES;                          // first tile of 128 rows
+    const uint32_t n_quads = (p.n_blocks + 3u) / 4u, all_st = (p.n_blocks + 7u) / 8u;
+    const uint32_t st0 = (uint32_t)((uint64_t)all_st * rank / p.splits);
+    const uint32_t n_st = (uint32_t)((uint64_t)all_st * (rank + 1u) / p.splits) - st0;   // at least one
+    const uint32_t b_stage = p.n * MP_STAGE_BYTES;
+    const uint32_t w_tiles = min(TILES, (p.rows + 127u) / 128u - tile0);                 // tiles that exist
 
     if (tid == 0) {
-        for (uint32_t s = 0; s < p.stages; ++s)
-            mbar_init(&bars->full[s], 1u + MP_ROW_WARPS + (DIGITS ? p.m : 0u)), mbar_init(&bars->empty[s], 1);
-        mbar_init(&bars->done, 1);
+        for (uint32_t s = 0; s < p.stages; ++s) mbar_init(&bars->full[s], 1u + (DIGITS ? p.m : 0u)), mbar_init(&bars->empty[s], 1);
+        mbar_init(&bars->done, MP_MMA_WARPS);
         bars->abort = 0;
         mbar_init_fence();
     }
@@ -153,184 +223,192 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // The weights too are read after the dependency wait below: a quantise call directly before this one may have
+    // written them.  Until then they are brought into L2, where a later write still reaches them: the launch before
+    // this one and the transfer from HBM overlap.
+    if (warp == 0 && elect_one()) {
+        for (uint32_t i = 0; i < w_tiles; ++i) {
+            for (uint32_t j = 0; j < min(n_st, MP_PREFETCH); ++j)
+                tma_prefetch_2d(&tm_w, (int32_t)((st0 + j) * MP_STAGE_BYTES), (int32_t)((tile0 + i) * MP_ROWS));
+            bulk_prefetch(p.w_scales + ((uint64_t)(tile0 + i) * n_quads + st0 * 2u) * MX_TILE_BYTES,
+                          min(n_st * 2u, n_quads - st0 * 2u) * MX_TILE_BYTES);
+        }
+    }
+    __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (p.splits > 1u) cluster_sync_all();   // every CTA of the cluster has started: its shared memory may be written
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = bars->tmem_base;
-    // An ordered launch (see axc_tuning.pdl).  The weights too are read after the wait: a quantise call directly
-    // before this one may have written them.
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // an ordered launch: see axc_tuning.pdl
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t issued = 0;
-            for (uint32_t st = 0; st < n_st && !bars->abort; ++st, ++issued) {
-                const uint32_t s = st % p.stages, ph = (st / p.stages) & 1u;
-                if (!mbar_wait(&bars->empty[s], ph ^ 1u, p.status)) {
-                    bars->abort = 1;
-                    break;
+        uint32_t s = 0, ph = 1, issued = 0;
+        for (; issued < n_st; ++issued) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->empty[s], ph, &bars->abort, p.status))) break;
+            if (elect_one()) {
+                const uint32_t st = st0 + issued, quad_bytes = min(2u, n_quads - st * 2u) * MX_TILE_BYTES;
+                mbar_expect_tx(&bars->full[s], w_tiles * (MP_W_BYTES + quad_bytes) + (DIGITS ? 0u : b_stage + quad_bytes));
+                for (uint32_t i = 0; i < w_tiles; ++i) {
+                    tma_load_2d(base + s * W_STAGE + i * MP_W_BYTES, &tm_w, (int32_t)(st * MP_STAGE_BYTES),
+                                (int32_t)((tile0 + i) * MP_ROWS), &bars->full[s]);
+                    bulk_g2s(sm + p.off_sfw + s * SFW_STAGE + i * 1024u,
+                             p.w_scales + ((uint64_t)(tile0 + i) * n_quads + st * 2u) * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
                 }
-                const uint32_t quads = min(2u, n_quads - st * 2u);   // scale tiles of this stage
-                uint32_t bytes = p.rows_per_cta * MP_STAGE_BYTES;
-                if (!DIGITS) bytes += p.n * MP_STAGE_BYTES + a_tiles * quads * MX_TILE_BYTES;
-                mbar_expect_tx(&bars->full[s], bytes);
-                tma_load_2d(base + s * p.a_stage, &tm_w, (int32_t)(st * MP_STAGE_BYTES), (int32_t)row0, &bars->full[s]);
-                if constexpr (!DIGITS) {
-                    tma_load_2d(base + p.off_b + s * p.b_stage, &tm_a, (int32_t)(st * MP_STAGE_BYTES), (int32_t)tok0, &bars->full[s]);
-                    for (uint32_t q = 0; q < a_tiles; ++q)
-                        bulk_g2s(sm + p.off_sfb + s * p.sfb_stage + q * 2u * MX_TILE_BYTES,
-                                 p.a_scales + ((uint64_t)(tok0 / 128u + q) * n_quads + st * 2u) * MX_TILE_BYTES,
-                                 quads * MX_TILE_BYTES, &bars->full[s]);
+                if (!DIGITS) {
+                    tma_load_2d(base + p.off_b + s * b_stage, &tm_a, (int32_t)(st * MP_STAGE_BYTES), 0, &bars->full[s]);
+                    bulk_g2s(sm + p.off_sfb + s * SFB_STAGE, p.a_scales + (uint64_t)st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
                 }
             }
-            // nothing may still be in flight towards this CTA's shared memory at exit
-            for (uint32_t j = issued > p.stages ? issued - p.stages : 0; j < issued; ++j)
-                (void)mbar_wait(&bars->full[j % p.stages], (j / p.stages) & 1u, p.status);
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            bool ok = true;
-            const uint32_t sf0 = tmem + p.n_acc * p.n;     // scale columns: 2 slots x 2 tiles x (4 + 4 * b_tiles)
-            for (uint32_t st = 0; st < n_st && !bars->abort; ++st) {
-                const uint32_t s = st % p.stages, ph = (st / p.stages) & 1u;
-                ok = mbar_wait(&bars->full[s], ph, p.status);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t slot = sf0 + (st & 1u) * (8u + 8u * b_tiles);
-                const uint32_t steps = min(4u, (p.n_blocks - st * 8u + 1u) / 2u);   // MMAs of 64 columns
-                for (uint32_t g = 0; g < (steps + 1u) / 2u; ++g) {
-                    scales_to_tmem(slot + g * 4u, base + p.off_sfa + s * 1024u + g * MX_TILE_BYTES);
-                    for (uint32_t q = 0; q < b_tiles; ++q)
-                        scales_to_tmem(slot + 8u + (g * b_tiles + q) * 4u,
-                                       base + p.off_sfb + s * p.sfb_stage + (q * 2u + g) * MX_TILE_BYTES);
-                }
-                const uint64_t ad = sw128_desc(base + s * p.a_stage), bd = sw128_desc(base + p.off_b + s * p.b_stage);
-                const uint32_t chain = min(st / MP_CHAIN, p.n_acc - 1u);
-                const uint32_t first = st == chain * MP_CHAIN;   // the chain's first stage overwrites its accumulator
-                for (uint32_t kk = 0; kk < steps; ++kk)          // 64 codes = 32 bytes = 2 descriptor units per step
-                    umma_mxf4(tmem + chain * p.n, ad + 2u * kk, bd + 2u * kk, mx_idesc(128u, p.n, (kk & 1u) * 2u),
-                              slot + (kk >> 1) * 4u, slot + 8u + (kk >> 1) * b_tiles * 4u, !(first && kk == 0u));
-                umma_commit(&bars->empty[s]);
-            }
-            if (!ok) bars->abort = 1;
-            umma_commit(&bars->done);     // accumulators complete (or nothing outstanding)
-        }
-    } else if (warp < 2u + MP_ROW_WARPS) {
-        // ---------------- scales of this CTA's rows: thread = row ----------------
-        const uint32_t r = (warp & 3u) * 32u + lane;     // also the TMEM lane of the epilogue
-        const uint64_t row = (uint64_t)row0 + r;
-        const bool mine = r < p.rows_per_cta && row < p.rows;
-        bool ok = true;
-        for (uint32_t st = 0; st < n_st && ok; ++st) {
-            const uint32_t s = st % p.stages, ph = (st / p.stages) & 1u;
-            uint32_t w[2] = {0, 0};
-#pragma unroll
-            for (uint32_t g = 0; g < 2; ++g)
-                if (mine && st * 2u + g < n_quads)
-                    w[g] = __ldg(reinterpret_cast<const uint32_t*>(p.w_scales + mx_scale_at(row, st * 2u + g, n_quads)));
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bars->empty[s], ph ^ 1u, p.status) && !bars->abort);
-            if (!ok) break;
-#pragma unroll
-            for (uint32_t g = 0; g < 2; ++g)
-                *reinterpret_cast<uint32_t*>(sm + p.off_sfa + s * 1024u + g * MX_TILE_BYTES + (r & 31u) * 16u + (r >> 5) * 4u) = w[g];
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // generic writes -> async proxy
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->full[s]);
+            if (++s == p.stages) s = 0, ph ^= 1u;
         }
-        if (!ok) bars->abort = 1;
+        // nothing may still be in flight towards this CTA's shared memory at exit
+        for (uint32_t j = issued > p.stages ? issued - p.stages : 0; j < issued; ++j)
+            (void)mbar_wait(&bars->full[j % p.stages], (j / p.stages) & 1u, p.status);
+    } else if (warp < MP_FIRST_X) {
+        // ---------------- MMA: warp `turn` takes the stages turn, turn + 2, ... into its accumulators ----------------
+        const uint32_t turn = warp - 1u;
+        if (elect_one()) {
+            const uint32_t sf0 = tmem + TILES * MP_MMA_WARPS * p.n, acc = tmem + turn * p.n;
+            const uint32_t idesc = mx_idesc(128u, p.n, 0u), idesc2 = mx_idesc(128u, p.n, 2u);
+            uint32_t s = turn % p.stages, ph = turn / p.stages;
+            for (uint32_t i = turn; i < n_st; i += MP_MMA_WARPS) {
+                if (!mbar_wait_or_abort(&bars->full[s], ph, &bars->abort, p.status)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t steps = min(4u, (p.n_blocks - (st0 + i) * 8u + 1u) / 2u);   // MMAs of 64 columns
+                const uint32_t sf = sf0 + s * SF_COLS, sfw = base + p.off_sfw + s * SFW_STAGE, sfb = base + p.off_sfb + s * SFB_STAGE;
+                const uint64_t wd = sw128_desc(base + s * W_STAGE), bd = sw128_desc(base + p.off_b + s * b_stage);
+#pragma unroll
+                for (uint32_t g = 0; g < 2u; ++g) {
+                    if (2u * g >= steps) break;
+                    scales_to_tmem(sf + g * 4u, sfb + g * MX_TILE_BYTES);
+#pragma unroll
+                    for (uint32_t t = 0; t < TILES; ++t)
+                        scales_to_tmem(sf + 8u + t * 8u + g * 4u, sfw + t * 1024u + g * MX_TILE_BYTES);
+                }
+#pragma unroll
+                for (uint32_t kk = 0; kk < 4u; ++kk) {           // 64 codes = 32 bytes = 2 descriptor units per step
+                    if (kk >= steps) break;
+#pragma unroll
+                    for (uint32_t t = 0; t < TILES; ++t)         // the first use of an accumulator overwrites it
+                        umma_mxf4(acc + t * MP_MMA_WARPS * p.n, wd + t * (MP_W_BYTES / 16u) + 2u * kk, bd + 2u * kk,
+                                  kk & 1u ? idesc2 : idesc, sf + 8u + t * 8u + (kk >> 1) * 4u, sf + (kk >> 1) * 4u, (i - turn) | kk);
+                }
+                umma_commit(&bars->empty[s]);
+                s += MP_MMA_WARPS;
+                while (s >= p.stages) s -= p.stages, ph ^= 1u;
+            }
+            umma_commit(&bars->done);     // this warp's accumulators are complete (or nothing is outstanding)
+        }
+    } else {
+        const uint32_t xw = warp - MP_FIRST_X;
+        if constexpr (DIGITS) {
+            // ---------------- digits of x: a warp takes 256 columns of one token, a lane 8 of them ----------------
+            // A place of the ring (stage and token) belongs to one warp, see launch().
+            const uint32_t takers = p.takers, units = xw < takers ? n_st * p.m : 0u;
+            float v[8];
+            if (xw < units) load_x(p, st0 + xw / p.m, xw % p.m, lane, v);
+            for (uint32_t u = xw; u < units; u += takers) {
+                const uint32_t i = u / p.m, t = u - i * p.m, s = i % p.stages, ph = (i / p.stages) & 1u;
+                uint32_t w[8], unit_bytes, nan;
+                split_x(v, lane, w, unit_bytes, nan);
+                const uint32_t next = u + takers;
+                if (next < units) load_x(p, st0 + next / p.m, next % p.m, lane, v);
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->empty[s], ph ^ 1u, &bars->abort, p.status))) break;
+                // row d of the token's eight rows; the 16-byte chunk j of a row sits at chunk j ^ (row & 7)
+                uint8_t* tile = sm + p.off_b + s * b_stage + t * 1024u;
+#pragma unroll
+                for (uint32_t d = 0; d < 8u; ++d)
+                    *reinterpret_cast<uint32_t*>(tile + d * 128u + (((lane >> 2) ^ d) << 4) + (lane & 3u) * 4u) = w[d];
+                // scales: lanes 0..7 write the first four blocks, lanes 16..23 the others; digit d is 8^d units
+                if ((lane & 15u) < 8u) {
+                    const uint32_t d = lane & 15u, n = t * 8u + d;
+                    *reinterpret_cast<uint32_t*>(sm + p.off_sfb + s * SFB_STAGE + (lane >> 4) * MX_TILE_BYTES + (n & 31u) * 16u +
+                                                 (n >> 5) * 4u) = (unit_bytes + 0x03030303u * d) | nan;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // generic writes -> async proxy
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->full[s]);
+            }
+        }
 
-        // ---------------- epilogue: TMEM lane = weight row ----------------
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bars->done, 0u, p.status) && !bars->abort);
+        // ---------------- epilogue: TMEM lane = weight row; partial sums to the CTA that finishes the row ----------------
+        const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->done, 0u, &bars->abort, p.status));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (ok) {
-            const uint32_t used = min(p.n_acc, (n_st + MP_CHAIN - 1u) / MP_CHAIN);
-            const uint32_t count = DIGITS ? p.m * 8u : min(p.n, p.m - tok0);
-            for (uint32_t c = 0; c < count; c += 8u) {
-                float sum[8] = {};
-                for (uint32_t a = 0; a < used; ++a) {
-                    uint32_t v[8];
-                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                                 : "r"(tmem + (((warp & 3u) * 32u) << 16) + a * p.n + c)
-                                 : "memory");
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            // two groups of four warps: one per tile, or taking turns at the columns of a single tile
+            const uint32_t grp = xw >> 2, quad = warp & 3u, t = TILES > 1u ? grp : 0u;
+            const uint32_t lr = t * MP_ROWS + quad * 32u + lane;          // row of the cluster's
+            const uint64_t row = (uint64_t)tile0 * MP_ROWS + lr;
+            const bool two = n_st > 1u;                                   // both issuing warps had a stage
+            const uint32_t taddr = tmem + ((quad * 32u) << 16) + t * MP_MMA_WARPS * p.n;
+            uint32_t dst = 0;
+            if (p.splits > 1u) {
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(base + p.off_red), "r"(lr >> p.per_shift));
+                const uint32_t slot = (rank << p.per_shift) | (lr & ((1u << p.per_shift) - 1u));   // [source][row]
+                dst += slot * red_row<DIGITS>(p.m) * 4u;
+            }
+            const uint32_t columns = DIGITS ? p.m * 8u : p.m;
+            for (uint32_t c = TILES > 1u ? 0u : grp * 8u; c < columns; c += TILES > 1u ? 8u : 16u) {
+                uint32_t r0[8], r1[8];
+                tmem_load8(taddr + c, r0);
+                tmem_load8(taddr + p.n + c, r1);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                float sum[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum[j] += __uint_as_float(v[j]);
-                }
-                if (!mine) continue;
-                if (DIGITS) {
-                    float y = sum[0];
+                for (int j = 0; j < 8; ++j) sum[j] = __uint_as_float(r0[j]) + (two ? __uint_as_float(r1[j]) : 0.0f);
+                if constexpr (DIGITS) {
+                    const float y = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+                    if (p.splits > 1u)
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + (c >> 3) * 4u), "f"(y) : "memory");
+                    else if (row < p.rows)
+                        put(reinterpret_cast<Out*>(p.out) + (uint64_t)(c >> 3) * p.rows + row, y);
+                } else if (p.splits > 1u) {
 #pragma unroll
-                    for (int j = 1; j < 8; ++j) y += sum[j];
-                    reinterpret_cast<float*>(p.out)[(uint64_t)(c >> 3) * p.rows + row] = y;
-                } else {
+                    for (int j = 0; j < 8; j += 4)
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c + j) * 4u), "f"(sum[j]),
+                                     "f"(sum[j + 1]), "f"(sum[j + 2]), "f"(sum[j + 3])
+                                     : "memory");
+                } else if (row < p.rows) {
+                    Out* out = reinterpret_cast<Out*>(p.out) + (uint64_t)c * p.rows + row;
 #pragma unroll
                     for (uint32_t j = 0; j < 8u; ++j)
-                        if (c + j < count) store_out(p, (uint64_t)(tok0 + c + j) * p.rows + row, sum[j]);
+                        if (c + j < columns) put(out + (uint64_t)j * p.rows, sum[j]);
                 }
             }
         }
-    } else if (DIGITS) {
-        // ---------------- digits of x: a warp takes 256 columns of one token, a lane 8 of them ----------------
-        const uint32_t k_total = p.n_blocks * 32u;
-        bool ok = true;
-        for (uint64_t u = warp - (2u + MP_ROW_WARPS); u < (uint64_t)n_st * p.m && ok; u += MP_X_WARPS) {
-            const uint32_t st = (uint32_t)(u / p.m), t = (uint32_t)(u - (uint64_t)st * p.m);
-            const uint32_t s = st % p.stages, ph = (st / p.stages) & 1u;
-            const uint32_t col = st * 256u + lane * 8u;
-            float v[8] = {};
-            if (col < k_total) {     // k_total is a multiple of 32
-                const float4* src = reinterpret_cast<const float4*>(p.x + (uint64_t)t * k_total + col);
-                const float4 a = __ldg(src), b = __ldg(src + 1);
-                v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-            }
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, (uint32_t)__float_as_int(v[i]) & 0x7FFFFFFFu);
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            // X = rn(x * 2^(22 - e)), e = exponent of the block's largest |x| plus one, so |X| <= 2^22; the unit of
-            // digit 0, with the half that a code counts, is 2^(e - 21): scale byte e - 21 + 127.  Blocks below
-            // 2^-105 keep the smallest unit 2^-127; 2^127 and above count as infinite (scale byte 255).
-            const uint32_t ex = top >> 23;                               // e = ex - 126
-            const bool bad = ex >= 254u;
-            const uint32_t unit = bad ? 0u : ex > 20u ? ex - 20u : 0u;   // scale byte of digit 0
-            // 2^(22 - e) = 2^(128 - unit): in two factors, since 2^128 is not a float
-            const float f1 = __int_as_float((int)((254u - unit) << 23));  // 2^(127 - unit)
-            uint32_t w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                // + 1.5 * 2^23 rounds to an integer in the low mantissa bits; + 4 in every octal digit, then ^ 4
-                // gives the digits -4..3 as three-bit two's complement fields
-                const float shifted = __fmaf_rn(v[i] * f1, 2.0f, 12582912.0f);
-                const uint32_t biased = (uint32_t)__float_as_int(shifted) + (0x00924924u - 0x4B400000u);
-                w[i] = spread_octal((bad ? 0x00924924u : biased) ^ 0x00924924u);
-            }
-            transpose_nibbles(w);
-            uint32_t sb = unit << (8u * ((lane >> 2) & 3u)), nan = bad ? 255u << (8u * ((lane >> 2) & 3u)) : 0u;
-            sb |= __shfl_xor_sync(0xFFFFFFFFu, sb, 4), nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, 4);
-            sb |= __shfl_xor_sync(0xFFFFFFFFu, sb, 8), nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, 8);
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bars->empty[s], ph ^ 1u, p.status) && !bars->abort);
-            if (!ok) break;
-            // row d of the token's eight rows; the 16-byte chunk j of a row sits at chunk j ^ (row & 7)
-            uint8_t* tile = sm + p.off_b + s * p.b_stage + t * 1024u;
-#pragma unroll
-            for (uint32_t d = 0; d < 8u; ++d)
-                *reinterpret_cast<uint32_t*>(tile + d * 128u + (((lane >> 2) ^ d) << 4) + (lane & 3u) * 4u) = digit_codes(w[d]);
-            // scales: lanes 0..7 write the first four blocks, lanes 16..23 the others; digit d is 8^d units
-            if ((lane & 15u) < 8u) {
-                const uint32_t d = lane & 15u, n = t * 8u + d;
-                *reinterpret_cast<uint32_t*>(sm + p.off_sfb + s * p.sfb_stage + (lane >> 4) * MX_TILE_BYTES + (n & 31u) * 16u +
-                                             (n >> 5) * 4u) = (sb + 0x03030303u * d) | nan;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->full[s]);
-        }
-        if (!ok) bars->abort = 1;
     }
 
+    if (p.splits > 1u) {
+        cluster_sync_all();
+        if (warp >= MP_FIRST_X) {
+            const uint32_t per = 1u << p.per_shift, pitch = red_row<DIGITS>(p.m);
+            const float* red = reinterpret_cast<const float*>(sm + p.off_red);
+            const uint64_t first = (uint64_t)tile0 * MP_ROWS + rank * per;
+            constexpr uint32_t WIDE = DIGITS ? 1u : 4u;            // neighbouring columns that a thread adds
+            for (uint32_t i = tid - MP_FIRST_X * 32u; i < (p.m + WIDE - 1u) / WIDE << p.per_shift; i += MP_X_WARPS * 32u) {
+                const uint32_t r = i & (per - 1u), c = (i >> p.per_shift) * WIDE;
+                float sum[WIDE] = {};
+                for (uint32_t k = 0; k < p.splits; ++k) {
+                    const float* src = red + ((k << p.per_shift) + r) * pitch + c;
+                    if constexpr (DIGITS) {
+                        sum[0] += src[0];
+                    } else {
+                        const float4 q = *reinterpret_cast<const float4*>(src);
+                        sum[0] += q.x, sum[1] += q.y, sum[2] += q.z, sum[3] += q.w;
+                    }
+                }
+                if (first + r < p.rows) {
+                    Out* out = reinterpret_cast<Out*>(p.out) + (uint64_t)c * p.rows + first + r;
+#pragma unroll
+                    for (uint32_t j = 0; j < WIDE; ++j)
+                        if (c + j < p.m) put(out + (uint64_t)j * p.rows, sum[j]);
+                }
+            }
+        }
+    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 1) {
@@ -339,42 +417,41 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     }
 }
 
-template <bool DIGITS>
-cudaError_t launch(const uint8_t* w_codes, const uint8_t* a_codes, MpArgs p, uint32_t smem_budget, uint32_t token_tiles,
-                   cudaStream_t stream) {
-    if (!tensor_map_encoder()) return cudaErrorNotSupported;
-    // Shared memory: W stages, B stages, row scales, B scales, barriers.  The MMA reads 128 rows of a W stage; the
-    // ones behind this CTA's rows are the next stage or what follows (their results are not used), and the region
-    // behind the last stage is larger than that.
-    const uint32_t b_tiles = (p.n + 127u) / 128u, n_st = (p.n_blocks + 7u) / 8u;
-    p.a_stage = (p.rows_per_cta + 7u) / 8u * 1024u;
-    p.b_stage = p.n * MP_STAGE_BYTES;
-    p.sfb_stage = b_tiles * 1024u;
-    const uint32_t per_stage = p.a_stage + p.b_stage + 1024u + p.sfb_stage;
-    const uint32_t fixed = 1024u + (uint32_t)sizeof(MpBars) + MP_ROWS * MP_STAGE_BYTES - p.a_stage;
-    uint32_t stages = (smem_budget - fixed) / per_stage;
+template <bool DIGITS, uint32_t TILES, typename Out>
+cudaError_t launch(const CUtensorMap& tm_w, const CUtensorMap& tm_a, MpArgs p, cudaStream_t stream) {
+    const uint32_t all_st = (p.n_blocks + 7u) / 8u;
+    const uint32_t share = (all_st + p.splits - 1u) / p.splits;     // the longest share of K, in stages
+    p.per_shift = 0;
+    while ((p.splits << p.per_shift) < TILES * MP_ROWS) ++p.per_shift;
+    // shared memory: W stages, B stages, scales of W and B, what the cluster sends, barriers
+    const uint32_t w_stage = TILES * MP_W_BYTES, b_stage = p.n * MP_STAGE_BYTES, sfw_stage = TILES * 1024u;
+    const uint32_t per_stage = w_stage + b_stage + sfw_stage + 1024u;
+    const uint32_t red = p.splits > 1u ? TILES * MP_ROWS * red_row<DIGITS>(p.m) * 4u : 0u;
+    const uint32_t fixed = 1024u + (uint32_t)sizeof(MpBars) + red;
+    uint32_t stages = (MP_SMEM_MAX - fixed) / per_stage;
     if (stages > MP_MAX_STAGES) stages = MP_MAX_STAGES;
-    if (stages > n_st) stages = n_st;
-    if (stages < 1u) stages = 1u;
-    p.stages = stages;
-    p.off_b = stages * p.a_stage;
-    p.off_sfa = p.off_b + stages * p.b_stage;
-    p.off_sfb = p.off_sfa + stages * 1024u;
-    p.off_bar = p.off_sfb + stages * p.sfb_stage;
-    const uint32_t smem = fixed + stages * per_stage;
-    // tensor memory: accumulators for chains of 4096 columns as far as they fit, two slots of scales
-    const uint32_t sf_cols = 2u * (8u + 8u * b_tiles);
-    uint32_t want = (n_st + MP_CHAIN - 1u) / MP_CHAIN;
+    if (stages > share) stages = share;
+    // Where the ring wraps, a place of it belongs to one issuing warp and, for each token, to one warp that splits x: a
+    // warp that waits for a place that another used last could take the parity of a phase still to come for its own.
+    p.takers = MP_X_WARPS;
+    if (stages < share) {
+        stages -= stages % MP_MMA_WARPS;
+        while (stages * p.m % p.takers) --p.takers;
+    }
+    // tensor memory: the accumulators, and a place of scales per stage
     uint32_t cols = 32u;
-    while (cols < p.n + sf_cols || (cols < 128u && cols < want * p.n + sf_cols)) cols *= 2u;
+    while (cols < TILES * MP_MMA_WARPS * p.n + stages * (8u * TILES + 8u)) cols *= 2u;
     p.tmem_cols = cols;
-    p.n_acc = (cols - sf_cols) / p.n;
-    if (p.n_acc > want) p.n_acc = want;
-    CUtensorMap tm_w, tm_a;
-    if (!mx_encode_codes(&tm_w, w_codes, p.rows, p.n_blocks, p.rows_per_cta)) return cudaErrorInvalidValue;
-    if (DIGITS) tm_a = tm_w;
-    else if (!mx_encode_codes(&tm_a, a_codes, p.m, p.n_blocks, p.n)) return cudaErrorInvalidValue;
-    auto kern = mx_product_kernel<DIGITS>;
+    p.stages = stages;
+    p.off_b = stages * w_stage;
+    p.off_sfw = p.off_b + stages * b_stage;
+    p.off_sfb = p.off_sfw + stages * sfw_stage;
+    p.off_red = p.off_sfb + stages * 1024u;
+    p.off_bar = p.off_red + red;
+    uint32_t smem = fixed + stages * per_stage;
+    const uint32_t least = MP_SMEM_SM / 512u * cols;                // an SM's CTAs never ask for more than 512 columns
+    if (smem < least) smem = least > MP_SMEM_MAX ? MP_SMEM_MAX : least;
+    auto kern = mx_product_kernel<DIGITS, TILES, Out>;
     {
         static std::mutex mu;
         static bool done[64] = {};
@@ -383,20 +460,33 @@ cudaError_t launch(const uint8_t* w_codes, const uint8_t* a_codes, MpArgs p, uin
         if (e != cudaSuccess) return e;
         std::lock_guard<std::mutex> lock(mu);
         if (dev < 0 || dev >= 64 || !done[dev]) {
-            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MP_SMEM_MAX);
             if (e != cudaSuccess) return e;
             if (dev >= 0 && dev < 64) done[dev] = true;
         }
     }
+    const uint32_t row_tiles = (p.rows + MP_ROWS - 1u) / MP_ROWS;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((p.rows + p.rows_per_cta - 1u) / p.rows_per_cta, token_tiles);
-    cfg.blockDim = dim3((2u + MP_ROW_WARPS + (DIGITS ? MP_X_WARPS : 0u)) * 32u);
+    cfg.gridDim = dim3((row_tiles + TILES - 1u) / TILES * p.splits);
+    cfg.blockDim = dim3(MP_THREADS);
     cfg.dynamicSmemBytes = smem, cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr, cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.splits, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = p.splits > 1u ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, tm_w, tm_a, p);
+}
+
+// CTAs per cluster: K is split as long as all CTAs fit the SMs at once and each keeps four stages (1024 columns).  A second
+// round of CTAs costs as much as the first (14336 x 4096, one token: 112 CTAs 7.8 us, 448 CTAs 14 us), and so do CTAs
+// that only start, send and stop (4096 x 4096: 4 splits of 4 stages 4.3 us, 8 of 2 stages 4.8 us, 1 of 16 7.5 us).
+uint32_t choose_splits(uint32_t groups, uint32_t n_blocks, uint32_t sms) {
+    const uint32_t st = (n_blocks + 7u) / 8u;
+    uint32_t splits = 1u;
+    while (splits < 8u && (uint64_t)groups * splits * 2u <= sms && st >= splits * 8u) splits *= 2u;
+    return splits;
 }
 
 }  // namespace
@@ -404,31 +494,43 @@ cudaError_t launch(const uint8_t* w_codes, const uint8_t* a_codes, MpArgs p, uin
 cudaError_t launch_mxfp4_matvec(const uint8_t* codes, const uint8_t* scales, const float* x, float* y, uint32_t m_tokens,
                                 uint32_t rows, uint32_t n_blocks, uint32_t* status, cudaStream_t stream, int sm_count) {
     if (m_tokens == 0 || rows == 0 || n_blocks == 0) return cudaSuccess;
+    if (!tensor_map_encoder()) return cudaErrorNotSupported;
     MpArgs p{};
     p.w_scales = scales, p.x = x, p.out = y, p.m = m_tokens, p.rows = rows, p.n_blocks = n_blocks, p.status = status;
-    p.out_type = (uint32_t)ElemType::F32;
     p.n = (m_tokens + 1u) / 2u * 16u;
-    // rows spread evenly over the SMs, in as many rounds as 128 rows per CTA make necessary
-    const uint32_t sms = (uint32_t)sm_count;
-    const uint32_t rounds = (uint32_t)(((uint64_t)rows + 128ull * sms - 1u) / (128ull * sms));
-    p.rows_per_cta = (uint32_t)(((uint64_t)rows + (uint64_t)rounds * sms - 1u) / ((uint64_t)rounds * sms));
-    return launch<true>(codes, nullptr, p, 110u * 1024u, 1u, stream);
+    CUtensorMap tm_w;
+    if (!mx_encode_codes(&tm_w, codes, rows, n_blocks, MP_ROWS)) return cudaErrorInvalidValue;
+    // Two tiles per CTA halve the work of splitting x, which every CTA does for its share of K.
+    const uint32_t row_tiles = (rows + MP_ROWS - 1u) / MP_ROWS;
+    if (row_tiles >= 8u) {
+        p.splits = choose_splits((row_tiles + 1u) / 2u, n_blocks, (uint32_t)sm_count);
+        return launch<true, 2, float>(tm_w, tm_w, p, stream);
+    }
+    p.splits = choose_splits(row_tiles, n_blocks, (uint32_t)sm_count);
+    return launch<true, 1, float>(tm_w, tm_w, p, stream);
 }
 
 cudaError_t launch_mxfp4_prefill(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* a_codes,
                                  const uint8_t* a_scales, void* c, ElemType type, uint32_t m_tokens, uint32_t n_rows,
                                  uint32_t n_blocks, uint32_t* status, cudaStream_t stream, int sm_count) {
     if (m_tokens == 0 || n_rows == 0 || n_blocks == 0) return cudaSuccess;
+    if (!tensor_map_encoder()) return cudaErrorNotSupported;
     if (m_tokens > 64u)
         return launch_mxfp4_gemm(w_codes, w_scales, a_codes, a_scales, c, type, m_tokens, n_rows, n_blocks, status, stream, sm_count);
     MpArgs p{};
     p.w_scales = w_scales, p.a_scales = a_scales, p.out = c, p.m = m_tokens, p.rows = n_rows, p.n_blocks = n_blocks;
-    p.status = status, p.out_type = (uint32_t)type;
-    p.n = m_tokens >= 256u ? 256u : (m_tokens + 15u) / 16u * 16u;
-    const uint32_t sms = (uint32_t)sm_count, token_tiles = (m_tokens + 255u) / 256u;
-    (void)sms;
-    p.rows_per_cta = 128u;
-    return launch<false>(w_codes, a_codes, p, 220u * 1024u, token_tiles, stream);
+    p.status = status;
+    p.n = (m_tokens + 15u) / 16u * 16u;
+    CUtensorMap tm_w, tm_a;
+    if (!mx_encode_codes(&tm_w, w_codes, n_rows, n_blocks, MP_ROWS) || !mx_encode_codes(&tm_a, a_codes, m_tokens, n_blocks, p.n))
+        return cudaErrorInvalidValue;
+    p.splits = choose_splits((n_rows + MP_ROWS - 1u) / MP_ROWS, n_blocks, (uint32_t)sm_count);
+    switch (type) {
+        case ElemType::F32: return launch<false, 1, float>(tm_w, tm_a, p, stream);
+        case ElemType::BF16: return launch<false, 1, __nv_bfloat16>(tm_w, tm_a, p, stream);
+        case ElemType::F16: return launch<false, 1, __half>(tm_w, tm_a, p, stream);
+    }
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace axc

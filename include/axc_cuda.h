@@ -335,8 +335,9 @@ int axc_cuda_mxfp4_dequant(const void* codes, const void* scales, void* w, uint3
 /* y[t][r] = sum_k W[r][k] * x[t][k] for m_tokens vectors x of n_blocks * 32 fp32 values, 1..8 of them.  x is not
  * rounded to 4 bits: within each block of 32 columns it is held as an integer of 23 bits with sign, relative to the
  * block's largest |x| (error at most 2^-22 of that), and the products with its base-8 digits are exact on the tensor
- * cores; sums are fp32.  Blocks whose largest |x| is below 2^-105 keep the absolute resolution 2^-128.  A block of x with a NaN, an infinity or a magnitude
- * of 2^127 or more makes every y of that token NaN.  n_blocks = 0 gives zeros.  *status (nullable) receives bit 0
+ * cores; sums are fp32.  Blocks whose largest |x| is below 2^-105 keep the absolute resolution
+ * 2^-127.  A block of x with a NaN, an infinity or a magnitude of 2^127 or more makes every y of that token NaN.
+ * n_blocks = 0 gives zeros.  *status (nullable) receives bit 0
  * if a bounded wait inside the kernel ran out. */
 #define AXC_MXFP4_MATVEC_TOKENS 8
 int axc_cuda_mxfp4_matvec(const void* codes, const void* scales, const float* x, float* y, uint32_t m_tokens, uint32_t rows,

@@ -318,7 +318,7 @@ def test_matvec_magnitudes_of_x(ops, power):
         x = (rng.uniform(0.5, 0.99, (1, 64)) * np.exp2(float(power) + 1)).astype(np.float32)
     y = ops.mxfp4_matvec(dev(codes), dev(tiles), dev(x), rows, nb).double().cpu().numpy().reshape(-1)
     x64 = x.astype(np.float64)
-    unit = max(2.0 ** -21 * np.abs(x64).max(), 2.0 ** -128)
+    unit = max(2.0 ** -21 * np.abs(x64).max(), 2.0 ** -127)
     fixed = unit / 2 * np.abs(w).sum(axis=1)
     mag = (np.abs(w) @ np.abs(x64).T)[:, 0]
     small = 64 * 2.0 ** -126                              # sums below the smallest normal number may be flushed
