@@ -19,7 +19,7 @@
 //                stage, and the commit that frees the stage.  With few columns an MMA is quick (32 cycles for its 4 KB of
 //                codes) and the issuing thread is the limit, about 550 cycles per stage: two take turns, each with an
 //                accumulator of its own (14336 x 4096, one token: 8.2 -> 7.8 us; four are no faster than two)
-//   warps 3..10  matvec: digits and scales of x, a warp taking 256 columns of one token at a time; then, in both, the
+//   warps 3...   matvec: digits and scales of x, a warp taking 256 columns of one token at a time; then, in both, the
 //                epilogue: every CTA holds partial sums of all its cluster's rows, sends those of each 1/splits of the
 //                rows to the CTA that finishes them (distributed shared memory), and adds what it got in rank order,
 //                so results do not depend on timing.
@@ -48,9 +48,12 @@ constexpr uint32_t MP_STAGE_BYTES = 128;            // one stage: 256 columns = 
 constexpr uint32_t MP_W_BYTES = MP_ROWS * MP_STAGE_BYTES;
 constexpr uint32_t MP_MAX_STAGES = 8;
 constexpr uint32_t MP_PREFETCH = 16;                // stages requested into L2 before the dependency wait
-constexpr uint32_t MP_MMA_WARPS = 2, MP_X_WARPS = 8;
-constexpr uint32_t MP_FIRST_X = 1 + MP_MMA_WARPS;   // warp
-constexpr uint32_t MP_THREADS = (MP_FIRST_X + MP_X_WARPS) * 32;
+constexpr uint32_t MP_MMA_WARPS = 2;
+constexpr uint32_t MP_FIRST_X = 1 + MP_MMA_WARPS;   // the first of the warps that split x and run the epilogue
+// A unit of 256 columns of one token takes such a warp about 1500 cycles, most of them waiting: with two tiles, where a
+// CTA has the SM to itself, 16 of them (8 tokens, 14336 x 4096: 12.4 us with 8 warps).
+__host__ __device__ constexpr uint32_t mp_x_warps(uint32_t tiles) { return 8u * tiles; }
+__host__ __device__ constexpr uint32_t mp_threads(uint32_t tiles) { return (MP_FIRST_X + mp_x_warps(tiles)) * 32u; }
 constexpr uint32_t MP_SMEM_SM = 228u * 1024u, MP_SMEM_MAX = 227u * 1024u;   // of an SM, of a CTA
 
 __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem_addr) {
@@ -192,9 +195,10 @@ __host__ __device__ __forceinline__ uint32_t red_row(uint32_t m) {
 }
 
 template <bool DIGITS, uint32_t TILES, typename Out>
-__global__ void __launch_bounds__(MP_THREADS, 1)
+__global__ void __launch_bounds__(mp_threads(TILES), 1)
 mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const MpArgs p) {
     constexpr uint32_t W_STAGE = TILES * MP_W_BYTES, SFW_STAGE = TILES * 1024u, SFB_STAGE = 1024u;
+    constexpr uint32_t X_WARPS = mp_x_warps(TILES);
     constexpr uint32_t SF_COLS = 8u * TILES + 8u;                  // scale columns of a place: B, then the tiles of W
     extern __shared__ uint8_t smem_dyn[];
     const uint32_t raw_addr = smem_u32(smem_dyn);
@@ -338,8 +342,8 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->done, 0u, &bars->abort, p.status));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (ok) {
-            // two groups of four warps: one per tile, or taking turns at the columns of a single tile
-            const uint32_t grp = xw >> 2, quad = warp & 3u, t = TILES > 1u ? grp : 0u;
+            // groups of four warps, two for each tile, that take turns at its columns
+            const uint32_t t = xw >> 3, grp = (xw >> 2) & 1u, quad = warp & 3u;
             const uint32_t lr = t * MP_ROWS + quad * 32u + lane;          // row of the cluster's
             const uint64_t row = (uint64_t)tile0 * MP_ROWS + lr;
             const bool two = n_st > 1u;                                   // both issuing warps had a stage
@@ -351,7 +355,7 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
                 dst += slot * red_row<DIGITS>(p.m) * 4u;
             }
             const uint32_t columns = DIGITS ? p.m * 8u : p.m;
-            for (uint32_t c = TILES > 1u ? 0u : grp * 8u; c < columns; c += TILES > 1u ? 8u : 16u) {
+            for (uint32_t c = grp * 8u; c < columns; c += 16u) {
                 uint32_t r0[8], r1[8];
                 tmem_load8(taddr + c, r0);
                 tmem_load8(taddr + p.n + c, r1);
@@ -388,7 +392,7 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
             const float* red = reinterpret_cast<const float*>(sm + p.off_red);
             const uint64_t first = (uint64_t)tile0 * MP_ROWS + rank * per;
             constexpr uint32_t WIDE = DIGITS ? 1u : 4u;            // neighbouring columns that a thread adds
-            for (uint32_t i = tid - MP_FIRST_X * 32u; i < (p.m + WIDE - 1u) / WIDE << p.per_shift; i += MP_X_WARPS * 32u) {
+            for (uint32_t i = tid - MP_FIRST_X * 32u; i < (p.m + WIDE - 1u) / WIDE << p.per_shift; i += X_WARPS * 32u) {
                 const uint32_t r = i & (per - 1u), c = (i >> p.per_shift) * WIDE;
                 float sum[WIDE] = {};
                 for (uint32_t k = 0; k < p.splits; ++k) {
@@ -433,7 +437,7 @@ cudaError_t launch(const CUtensorMap& tm_w, const CUtensorMap& tm_a, MpArgs p, c
     if (stages > share) stages = share;
     // Where the ring wraps, a place of it belongs to one issuing warp and, for each token, to one warp that splits x: a
     // warp that waits for a place that another used last could take the parity of a phase still to come for its own.
-    p.takers = MP_X_WARPS;
+    p.takers = mp_x_warps(TILES);
     if (stages < share) {
         stages -= stages % MP_MMA_WARPS;
         while (stages * p.m % p.takers) --p.takers;
@@ -468,7 +472,7 @@ cudaError_t launch(const CUtensorMap& tm_w, const CUtensorMap& tm_a, MpArgs p, c
     const uint32_t row_tiles = (p.rows + MP_ROWS - 1u) / MP_ROWS;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((row_tiles + TILES - 1u) / TILES * p.splits);
-    cfg.blockDim = dim3(MP_THREADS);
+    cfg.blockDim = dim3(mp_threads(TILES));
     cfg.dynamicSmemBytes = smem, cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
