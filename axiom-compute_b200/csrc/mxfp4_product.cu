@@ -483,14 +483,16 @@ cudaError_t launch(const CUtensorMap& tm_w, const CUtensorMap& tm_a, MpArgs p, c
     return cudaLaunchKernelEx(&cfg, kern, tm_w, tm_a, p);
 }
 
-// CTAs per cluster: K is split as long as all CTAs fit the SMs at once and each keeps four stages (1024 columns).  A second
-// round of CTAs costs as much as the first (14336 x 4096, one token: 112 CTAs 7.8 us, 448 CTAs 14 us), and so do CTAs
-// that only start, send and stop (4096 x 4096: 4 splits of 4 stages 4.3 us, 8 of 2 stages 4.8 us, 1 of 16 7.5 us).
+// CTAs per cluster: K is split as long as each CTA keeps four stages (1024 columns) and all clusters run at once.  A second
+// round of CTAs costs as much as the first (14336 x 4096, one token: 112 CTAs 7.6 us, 224 CTAs 11.5 us), and clusters of 4
+// and 8 do not reach every SM (15 clusters of 8 on 148 SMs; 2000 x 16000, three tokens: 64 CTAs in clusters of 8 7.8 us, 128
+// CTAs 12.6 us).
 uint32_t choose_splits(uint32_t groups, uint32_t n_blocks, uint32_t sms) {
     const uint32_t st = (n_blocks + 7u) / 8u;
-    uint32_t splits = 1u;
-    while (splits < 8u && (uint64_t)groups * splits * 2u <= sms && st >= splits * 8u) splits *= 2u;
-    return splits;
+    const uint64_t most[4] = {sms, sms, sms * 7u / 8u, sms * 3u / 4u};   // CTAs that run at once in clusters of 1, 2, 4, 8
+    uint32_t shift = 0;
+    while (shift < 3u && ((uint64_t)groups << (shift + 1u)) <= most[shift + 1u] && st >= 8u << shift) ++shift;
+    return 1u << shift;
 }
 
 }  // namespace
@@ -504,9 +506,11 @@ cudaError_t launch_mxfp4_matvec(const uint8_t* codes, const uint8_t* scales, con
     p.n = (m_tokens + 1u) / 2u * 16u;
     CUtensorMap tm_w;
     if (!mx_encode_codes(&tm_w, codes, rows, n_blocks, MP_ROWS)) return cudaErrorInvalidValue;
-    // Two tiles per CTA halve the work of splitting x, which every CTA does for its share of K.
+    // Two tiles per CTA halve the work of splitting x, which every CTA does for its share of K (one token, 8192 x 8192: 8.3
+    // us, one tile 9.4 us; 57344 x 8192: 43 us, 50 us).  Rows of three stages or less are too short for it: 40000 x 512
+    // 6.7 us, one tile 5.7 us.
     const uint32_t row_tiles = (rows + MP_ROWS - 1u) / MP_ROWS;
-    if (row_tiles >= 8u) {
+    if (row_tiles >= 8u && n_blocks > 24u) {
         p.splits = choose_splits((row_tiles + 1u) / 2u, n_blocks, (uint32_t)sm_count);
         return launch<true, 2, float>(tm_w, tm_w, p, stream);
     }
@@ -528,11 +532,14 @@ cudaError_t launch_mxfp4_prefill(const uint8_t* w_codes, const uint8_t* w_scales
     CUtensorMap tm_w, tm_a;
     if (!mx_encode_codes(&tm_w, w_codes, n_rows, n_blocks, MP_ROWS) || !mx_encode_codes(&tm_a, a_codes, m_tokens, n_blocks, p.n))
         return cudaErrorInvalidValue;
-    p.splits = choose_splits((n_rows + MP_ROWS - 1u) / MP_ROWS, n_blocks, (uint32_t)sm_count);
+    // Two tiles per CTA where one each would need a second round of CTAs: 28672 x 3200, 64 tokens 15.9 -> 12.1 us.
+    const uint32_t row_tiles = (n_rows + MP_ROWS - 1u) / MP_ROWS;
+    const bool two = row_tiles > (uint32_t)sm_count;
+    p.splits = choose_splits(two ? (row_tiles + 1u) / 2u : row_tiles, n_blocks, (uint32_t)sm_count);
     switch (type) {
-        case ElemType::F32: return launch<false, 1, float>(tm_w, tm_a, p, stream);
-        case ElemType::BF16: return launch<false, 1, __nv_bfloat16>(tm_w, tm_a, p, stream);
-        case ElemType::F16: return launch<false, 1, __half>(tm_w, tm_a, p, stream);
+        case ElemType::F32: return two ? launch<false, 2, float>(tm_w, tm_a, p, stream) : launch<false, 1, float>(tm_w, tm_a, p, stream);
+        case ElemType::BF16: return two ? launch<false, 2, __nv_bfloat16>(tm_w, tm_a, p, stream) : launch<false, 1, __nv_bfloat16>(tm_w, tm_a, p, stream);
+        case ElemType::F16: return two ? launch<false, 2, __half>(tm_w, tm_a, p, stream) : launch<false, 1, __half>(tm_w, tm_a, p, stream);
     }
     return cudaErrorInvalidValue;
 }
