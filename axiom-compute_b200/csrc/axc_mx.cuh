@@ -23,6 +23,10 @@ __host__ __device__ __forceinline__ uint64_t mx_scale_bytes(uint64_t rows, uint6
     return (rows + 127u) / 128u * ((n_blocks + 3u) / 4u) * MX_TILE_BYTES;
 }
 
+// Kernels that stream rows give a warp one segment of 256 columns at a time up to this many segments (two rounds of the
+// warps of all SMs), and four beyond.
+constexpr uint64_t SMALL_SEGMENTS = 148u * 64u * 2u;
+
 // Byte offset of the scales of blocks 4 * quad .. 4 * quad + 3 of a row; n_quads = ceil(n_blocks / 4).
 __host__ __device__ __forceinline__ uint64_t mx_scale_at(uint64_t row, uint32_t quad, uint32_t n_quads) {
     return ((row >> 7) * n_quads + quad) * MX_TILE_BYTES + (row & 31u) * 16u + ((row >> 5) & 3u) * 4u;
@@ -45,18 +49,17 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 
-// Eight consecutive output values, rounded to nearest even, in one or two 16-byte stores.
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+// Consecutive output values in one 16-byte store, rounded to nearest even.
+__device__ __forceinline__ void store16(float* p, const float (&v)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+__device__ __forceinline__ void store16(__nv_bfloat16* p, const float (&v)[8]) {
     __nv_bfloat162 h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
 }
-__device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
+__device__ __forceinline__ void store16(__half* p, const float (&v)[8]) {
     __half2 h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);

@@ -5,94 +5,140 @@
 // the even code, larger magnitudes to 6.  The product x * 2^-e is exact (a power of two between 2^-125 and 2^127),
 // so each value is rounded once.  A block that holds a NaN or an infinity gets the NaN scale and zero codes.
 //
-// One pass over x, bound by HBM: 2 or 4 bytes read and 17/32 byte written per value.  A warp takes 256 columns of a
-// row, a lane 8 of them (one 16-byte load of 16-bit values): the block maximum is two shuffles over four lanes, the
-// codes of a warp are 128 contiguous bytes, and its scales are two 4-byte words.
+// One pass over x, bound by HBM: 2 or 4 bytes read and 17/32 byte written per value.  A warp takes segments of 256 columns
+// of a row, a lane 8 neighbouring columns of each (one 16-byte load of 16-bit values): the block maximum is two shuffles
+// over four lanes, the codes of a segment are 128 contiguous bytes, and its scales are two 4-byte words.  Where there is
+// work for it, four segments are under way at a time.
 #include "axc_kernels.h"
 #include "axc_mx.cuh"
 
 namespace axc {
 namespace {
 
-__device__ __forceinline__ float widen(float v) { return v; }
-__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
+// Eight values as they lie in memory, the largest magnitude among them as the bits of an fp32 (NaN and infinity compare
+// above every finite value), and the values as fp32.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p));
-    const T* h = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = widen(h[i]);
-}
+struct Eight;
 
-// Two values to two codes in one byte, the first in the low nibble: nearest even, saturating.
-__device__ __forceinline__ uint32_t code_pair(float lo, float hi) {
+template <>
+struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+    __device__ __forceinline__ void load_edge(const float* p, uint32_t count) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) v[i] = i < count ? __ldg(p + i) : 0.0f;
+    }
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t t = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t = max(t, (uint32_t)__float_as_int(v[i]) & 0x7FFFFFFFu);
+        return t;
+    }
+    __device__ __forceinline__ float value(int i) const { return v[i]; }
+};
+
+// 16-bit types: the magnitudes of two values are compared in one instruction.
+struct EightHalves {
+    uint32_t w[4];
+    template <typename T>
+    __device__ __forceinline__ void load(const T* p) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    }
+    template <typename T>
+    __device__ __forceinline__ void load_edge(const T* p, uint32_t count) {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i)
+            w[i] = (2u * i < count ? (uint32_t)__ldg(h + 2u * i) : 0u) | (2u * i + 1u < count ? (uint32_t)__ldg(h + 2u * i + 1u) << 16 : 0u);
+    }
+    __device__ __forceinline__ uint32_t top16() const {
+        const uint32_t t = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+        return max(t & 0xFFFFu, t >> 16);
+    }
+};
+template <>
+struct Eight<__nv_bfloat16> : EightHalves {
+    __device__ __forceinline__ uint32_t top() const { return top16() << 16; }
+    __device__ __forceinline__ float value(int i) const { return __int_as_float((int)(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16)); }
+};
+template <>
+struct Eight<__half> : EightHalves {
+    __device__ __forceinline__ uint32_t top() const { return (uint32_t)__float_as_int(f16_bits_to_f32(top16())) & 0x7FFFFFFFu; }
+    __device__ __forceinline__ float value(int i) const { return f16_bits_to_f32(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xFFFFu); }
+};
+
+// Eight values to eight codes, the first in the lowest nibble: nearest even, saturating.
+template <typename T>
+__device__ __forceinline__ uint32_t codes_of(const Eight<T>& x, float inv) {
     uint32_t r;
-    asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\tcvt.u32.u8 %0, b;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r)
+        : "f"(x.value(0) * inv), "f"(x.value(1) * inv), "f"(x.value(2) * inv), "f"(x.value(3) * inv), "f"(x.value(4) * inv),
+          "f"(x.value(5) * inv), "f"(x.value(6) * inv), "f"(x.value(7) * inv));
     return r;
 }
 
-template <typename T>
+template <typename T, uint32_t SEGS>   // segments of 256 columns that a warp has under way
 __global__ void __launch_bounds__(256)
 mxfp4_quantize_kernel(const T* __restrict__ x, uint64_t row_stride, uint32_t rows, uint32_t cols, uint32_t n_blocks,
-                      uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint32_t n_seg, uint64_t n_items, int wide) {
+                      uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint32_t n_groups, uint64_t n_items, int wide) {
     asm volatile("griddepcontrol.wait;" ::: "memory");   // an ordered launch: see axc_tuning.pdl
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t n_quads = (n_blocks + 3u) / 4u;
     const uint64_t warps = (uint64_t)gridDim.x * (blockDim.x >> 5);
     for (uint64_t item = (uint64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); item < n_items; item += warps) {
-        const uint64_t row = item / n_seg;
-        const uint32_t seg = (uint32_t)(item - row * n_seg);
-        const uint32_t col = seg * 256u + lane * 8u;
-        float v[8] = {};
-        if (row < rows) {
-            const T* src = x + row * row_stride + col;
-            if (wide && col + 8u <= cols) {
-                load8(src, v);
-            } else {
+        const uint64_t row = n_groups == 1u ? item : item >> 32 ? item / n_groups : (uint32_t)item / n_groups;
+        const uint32_t seg0 = (uint32_t)(item - row * n_groups) * SEGS;
+        Eight<T> v[SEGS];
+        const T* src = x + row * row_stride;
+        const uint32_t end = row < rows ? cols : 0u;             // rows that only fill up a tile of scales read as zero
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i)
-                    if (col + i < cols) v[i] = widen(src[i]);
-            }
+        for (uint32_t k = 0; k < SEGS; ++k) {
+            const uint32_t col = (seg0 + k) * 256u + lane * 8u;
+            if (wide && col + 8u <= end) v[k].load(src + col);
+            else v[k].load_edge(src + col, end > col ? end - col : 0u);
         }
-        // the largest magnitude as bits: NaN and infinity compare above every finite value
-        uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, (uint32_t)__float_as_int(v[i]) & 0x7FFFFFFFu);
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        const uint32_t ex = top >> 23;                       // biased exponent; 0 for zero and subnormal
-        const bool bad = ex == 255u;
-        const uint32_t byte = bad ? 255u : ex > 2u ? ex - 2u : 0u;
-        // 2^-(byte - 127) = 2^(127 - byte), byte <= 252
-        const float inv = __int_as_float((int)((254u - (bad ? 127u : byte)) << 23));
-        uint32_t word = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) word |= code_pair(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
-        if (bad) word = 0;
-        const uint32_t block = seg * 8u + (lane >> 2);
-        if (row < rows && block < n_blocks)
-            *reinterpret_cast<uint32_t*>(codes + (row * n_blocks + block) * MX_BLOCK_BYTES + (lane & 3u) * 4u) = word;
-        // the four scales of 16 lanes in one word; blocks and rows that only fill up a tile are zero
-        uint32_t s = row < rows && block < n_blocks ? byte << (8u * ((lane >> 2) & 3u)) : 0u;
-        s |= __shfl_xor_sync(0xFFFFFFFFu, s, 4);
-        s |= __shfl_xor_sync(0xFFFFFFFFu, s, 8);
-        const uint32_t quad = seg * 2u + (lane >> 4);
-        if ((lane & 15u) == 0u && quad < n_quads) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(row, quad, n_quads)) = s;
+        for (uint32_t k = 0; k < SEGS; ++k) {
+            const uint32_t seg = seg0 + k;
+            if (seg * 8u >= n_blocks) break;
+            uint32_t top = v[k].top();
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            const uint32_t ex = top >> 23;                       // biased exponent; 0 for zero and subnormal
+            const bool bad = ex == 255u;
+            uint32_t byte = max(ex, 2u) - 2u;
+            const float inv = __int_as_float((int)((254u - byte) << 23));   // 2^-(byte - 127)
+            uint32_t word = codes_of(v[k], inv);
+            if (bad) word = 0u, byte = 255u;
+            const uint32_t block = seg * 8u + (lane >> 2);
+            const bool real = row < rows && block < n_blocks;
+            if (real) *reinterpret_cast<uint32_t*>(codes + (row * n_blocks + block) * MX_BLOCK_BYTES + (lane & 3u) * 4u) = word;
+            // the four scales of 16 lanes in one word; blocks and rows that only fill up a tile are zero
+            uint32_t s = real ? byte << (8u * ((lane >> 2) & 3u)) : 0u;
+            s |= __shfl_xor_sync(0xFFFFFFFFu, s, 4);
+            s |= __shfl_xor_sync(0xFFFFFFFFu, s, 8);
+            const uint32_t quad = seg * 2u + (lane >> 4);
+            if ((lane & 15u) == 0u && quad < n_quads) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(row, quad, n_quads)) = s;
+        }
     }
 }
 
-template <typename T>
-cudaError_t launch(const void* x, uint64_t row_stride, uint32_t rows, uint32_t cols, uint8_t* codes, uint8_t* scales,
+template <typename T, uint32_t SEGS>
+cudaError_t launch_segs(const void* x, uint64_t row_stride, uint32_t rows, uint32_t cols, uint8_t* codes, uint8_t* scales,
                    cudaStream_t stream) {
-    const uint32_t n_blocks = (cols + 31u) / 32u, n_seg = (n_blocks + 7u) / 8u;
-    const uint64_t n_items = ((uint64_t)rows + 127u) / 128u * 128u * n_seg;
+    const uint32_t n_blocks = (cols + 31u) / 32u, n_groups = (n_blocks + SEGS * 8u - 1u) / (SEGS * 8u);
+    const uint64_t n_items = ((uint64_t)rows + 127u) / 128u * 128u * n_groups;
     const uint64_t want = (n_items + 7u) / 8u;
     const int wide = ((uintptr_t)x & 15u) == 0 && (row_stride * sizeof(T)) % 16u == 0;
     cudaLaunchConfig_t cfg{};
@@ -101,8 +147,16 @@ cudaError_t launch(const void* x, uint64_t row_stride, uint32_t rows, uint32_t c
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr, cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, mxfp4_quantize_kernel<T>, (const T*)x, row_stride, rows, cols, n_blocks, codes, scales,
-                              n_seg, n_items, wide);
+    return cudaLaunchKernelEx(&cfg, mxfp4_quantize_kernel<T, SEGS>, (const T*)x, row_stride, rows, cols, n_blocks, codes, scales,
+                              n_groups, n_items, wide);
+}
+
+template <typename T>
+cudaError_t launch(const void* x, uint64_t row_stride, uint32_t rows, uint32_t cols, uint8_t* codes, uint8_t* scales,
+                   cudaStream_t stream) {
+    const uint64_t segs = ((uint64_t)rows + 127u) / 128u * 128u * ((cols + 255u) / 256u);
+    return segs <= SMALL_SEGMENTS ? launch_segs<T, 1>(x, row_stride, rows, cols, codes, scales, stream)
+                                  : launch_segs<T, 4>(x, row_stride, rows, cols, codes, scales, stream);
 }
 
 }  // namespace
