@@ -142,7 +142,7 @@ cudaError_t launch_segs(const void* x, uint64_t row_stride, uint32_t rows, uint3
     const uint64_t want = (n_items + 7u) / 8u;
     const int wide = ((uintptr_t)x & 15u) == 0 && (row_stride * sizeof(T)) % 16u == 0;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(want < 148u * 8u ? want : 148u * 8u)), cfg.blockDim = dim3(256), cfg.stream = stream;
+    cfg.gridDim = dim3((unsigned)(want < (1u << 30) ? want : (1u << 30))), cfg.blockDim = dim3(256), cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

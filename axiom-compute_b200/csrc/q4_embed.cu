@@ -169,7 +169,7 @@ cudaError_t launch_segs(const RowsArgs& a, cudaStream_t stream) {
     const uint64_t n_items = (uint64_t)a.n_ids * n_groups;
     const uint64_t want = (n_items + 7u) / 8u;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(want < 148u * 8u ? want : 148u * 8u)), cfg.blockDim = dim3(256), cfg.stream = stream;
+    cfg.gridDim = dim3((unsigned)(want < (1u << 30) ? want : (1u << 30))), cfg.blockDim = dim3(256), cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
