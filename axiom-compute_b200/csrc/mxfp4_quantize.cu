@@ -100,18 +100,21 @@ mxfp4_quantize_kernel(const T* __restrict__ x, uint64_t row_stride, uint32_t row
         const uint64_t row = n_groups == 1u ? item : item >> 32 ? item / n_groups : (uint32_t)item / n_groups;
         const uint32_t seg0 = (uint32_t)(item - row * n_groups) * SEGS;
         Eight<T> v[SEGS];
-        const T* src = x + row * row_stride;
+        const uint32_t col0 = seg0 * 256u + lane * 8u;
+        const T* src = x + row * row_stride + col0;
         const uint32_t end = row < rows ? cols : 0u;             // rows that only fill up a tile of scales read as zero
+        const uint32_t left = end > col0 ? end - col0 : 0u;
 #pragma unroll
         for (uint32_t k = 0; k < SEGS; ++k) {
-            const uint32_t col = (seg0 + k) * 256u + lane * 8u;
-            if (wide && col + 8u <= end) v[k].load(src + col);
-            else v[k].load_edge(src + col, end > col ? end - col : 0u);
+            if (wide && k * 256u + 8u <= left) v[k].load(src + k * 256u);
+            else v[k].load_edge(src + k * 256u, left > k * 256u ? left - k * 256u : 0u);
         }
+        // block seg0 * 8 + k * 8 + lane / 4 of the row; how many of them k runs over
+        const uint32_t block0 = seg0 * 8u + (lane >> 2), blocks = row < rows && n_blocks > block0 ? n_blocks - block0 : 0u;
+        uint8_t* dst = codes + (row * n_blocks + block0) * MX_BLOCK_BYTES + (lane & 3u) * 4u;
+        uint32_t bytes = 0;                                      // scale of block k in byte k; zero where there is none
 #pragma unroll
         for (uint32_t k = 0; k < SEGS; ++k) {
-            const uint32_t seg = seg0 + k;
-            if (seg * 8u >= n_blocks) break;
             uint32_t top = v[k].top();
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
@@ -121,16 +124,31 @@ mxfp4_quantize_kernel(const T* __restrict__ x, uint64_t row_stride, uint32_t row
             const float inv = __int_as_float((int)((254u - byte) << 23));   // 2^-(byte - 127)
             uint32_t word = codes_of(v[k], inv);
             if (bad) word = 0u, byte = 255u;
-            const uint32_t block = seg * 8u + (lane >> 2);
-            const bool real = row < rows && block < n_blocks;
-            if (real) *reinterpret_cast<uint32_t*>(codes + (row * n_blocks + block) * MX_BLOCK_BYTES + (lane & 3u) * 4u) = word;
-            // the four scales of 16 lanes in one word; blocks and rows that only fill up a tile are zero
-            uint32_t s = real ? byte << (8u * ((lane >> 2) & 3u)) : 0u;
-            s |= __shfl_xor_sync(0xFFFFFFFFu, s, 4);
-            s |= __shfl_xor_sync(0xFFFFFFFFu, s, 8);
-            const uint32_t quad = seg * 2u + (lane >> 4);
-            if ((lane & 15u) == 0u && quad < n_quads) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(row, quad, n_quads)) = s;
+            if (k * 8u < blocks) {
+                *reinterpret_cast<uint32_t*>(dst + k * 8u * MX_BLOCK_BYTES) = word;
+                bytes |= byte << (8u * k);
+            }
         }
+        // The scales of four neighbouring blocks, which lie in lanes four apart, make one word.
+        const uint32_t g = (lane >> 2) & 3u, half = lane >> 4;
+        uint32_t word, seg = seg0;
+        bool writes;
+        if constexpr (SEGS == 4) {
+            // 4 x 4 bytes turned over between the lanes g = 0..3: lane g ends up with segment g
+            const uint32_t q = __shfl_xor_sync(0xFFFFFFFFu, bytes, 8);
+            bytes = __byte_perm(bytes, q, g & 2u ? 0x3276 : 0x5410);
+            const uint32_t r = __shfl_xor_sync(0xFFFFFFFFu, bytes, 4);
+            word = __byte_perm(bytes, r, g & 1u ? 0x3715 : 0x6240);
+            seg += g;
+            writes = (lane & 3u) == 0u;
+        } else {
+            word = bytes << (8u * g);
+            word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
+            word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
+            writes = (lane & 15u) == 0u;
+        }
+        const uint32_t quad = seg * 2u + half;
+        if (writes && quad < n_quads) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(row, quad, n_quads)) = word;
     }
 }
 
