@@ -169,14 +169,21 @@ def _count(value, name: str, least: int = 0) -> int:
     return value
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None)          # what torch.cuda.current_device() and
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)    # current_stream(i).cuda_stream read
+
+
+def _lib():
+    return _ffi._lib or _ffi.lib()
+
+
 def _ptr(t: torch.Tensor, dtype, name: str, min_elems: int, device: int) -> int:
     """``_chk``, and on CUDA device `device`.  (A small call is bound by the host: the checks that pass are kept to a
     few attribute reads.)"""
-    if t.dtype is dtype and t.is_cuda and t.is_contiguous() and t.numel() >= min_elems:
-        if t.get_device() != device:
-            raise ValueError(f"{name} is on {t.device}, the first operand on cuda:{device}")
+    if t.dtype is dtype and t.get_device() == device and t.is_contiguous() and t.numel() >= min_elems:
         return t.data_ptr()
-    return _chk(t, dtype, name, min_elems)      # says what is wrong
+    _chk(t, dtype, name, min_elems)      # says what is wrong
+    raise ValueError(f"{name} is on {t.device}, the first operand on cuda:{device}")
 
 
 def _device_of(t: torch.Tensor, name: str) -> int:
@@ -185,14 +192,13 @@ def _device_of(t: torch.Tensor, name: str) -> int:
     return t.get_device()
 
 
-def _launch(device: int, fn, *args) -> None:
-    """fn(*args[:-1], stream, *args[-1]) on the current stream of CUDA device `device`."""
-    stream = torch._C._cuda_getCurrentRawStream(device)
-    if device == torch._C._cuda_getDevice():
-        rc = fn(*args[:-1], stream, *args[-1])
+def _call(device: int, fn, *args) -> None:
+    """fn(*args) with CUDA device `device` current; a status other than OK raises."""
+    if device == _current_device():
+        rc = fn(*args)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args[:-1], stream, *args[-1])
+            rc = fn(*args)
     if rc:
         _raise_for(rc)
 
@@ -237,11 +243,11 @@ def mxfp4_quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales
     _count(rows, "rows"), _count(cols, "cols")
     n_blocks = (cols + 31) // 32
     if codes is None:
-        codes = x.new_empty((rows, n_blocks * MX_BLOCK_BYTES), dtype=torch.uint8)
+        codes = torch.empty(rows, n_blocks * MX_BLOCK_BYTES, dtype=torch.uint8, device=x.device)
     if scales is None:
-        scales = x.new_empty(_tile_bytes(rows, n_blocks), dtype=torch.uint8)
+        scales = torch.empty(_tile_bytes(rows, n_blocks), dtype=torch.uint8, device=x.device)
     cp, sp = _mx_operand(codes, scales, rows, n_blocks, "", device)
-    _launch(device, _ffi.lib().axc_cuda_mxfp4_quantize, x.data_ptr(), xt, stride, rows, cols, cp, sp, ())
+    _call(device, _lib().axc_cuda_mxfp4_quantize, x.data_ptr(), xt, stride, rows, cols, cp, sp, _raw_stream(device))
     return codes, scales
 
 
@@ -254,9 +260,9 @@ def mxfp4_dequant(codes: torch.Tensor, scales: torch.Tensor, rows: int, n_blocks
     cp, sp = _mx_operand(codes, scales, rows, n_blocks, "", device)
     wt = _float_type(out_dtype, "out_dtype")
     if w is None:
-        w = codes.new_empty((rows, n_blocks * MX_BLOCK_ELEMS), dtype=out_dtype)
+        w = torch.empty(rows, n_blocks * MX_BLOCK_ELEMS, dtype=out_dtype, device=codes.device)
     wp = _ptr(w, out_dtype, "w", rows * n_blocks * MX_BLOCK_ELEMS, device)
-    _launch(device, _ffi.lib().axc_cuda_mxfp4_dequant, cp, sp, wp, wt, rows, n_blocks, ())
+    _call(device, _lib().axc_cuda_mxfp4_dequant, cp, sp, wp, wt, rows, n_blocks, _raw_stream(device))
     return w
 
 
@@ -270,10 +276,11 @@ def mxfp4_matvec(codes: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, row
     cp, sp = _mx_operand(codes, scales, rows, n_blocks, "", device)
     xp = _ptr(x, torch.float32, "x", m_tokens * n_blocks * MX_BLOCK_ELEMS, device)
     if y is None:
-        y = x.new_empty((m_tokens, rows) if m_tokens > 1 or x.dim() > 1 else rows)
+        y = torch.empty(rows, dtype=torch.float32, device=x.device) if m_tokens == 1 and x.dim() <= 1 else \
+            torch.empty(m_tokens, rows, dtype=torch.float32, device=x.device)
     yp = _ptr(y, torch.float32, "y", m_tokens * rows, device)
-    _launch(device, _ffi.lib().axc_cuda_mxfp4_matvec, cp, sp, xp, yp, m_tokens, rows, n_blocks,
-            (_status_ptr(status, device),))
+    _call(device, _lib().axc_cuda_mxfp4_matvec, cp, sp, xp, yp, m_tokens, rows, n_blocks, _raw_stream(device),
+          _status_ptr(status, device))
     return y
 
 
@@ -288,10 +295,10 @@ def mxfp4_prefill(w_codes: torch.Tensor, w_scales: torch.Tensor, a_codes: torch.
     ap, asp = _mx_operand(a_codes, a_scales, m_tokens, n_blocks, "a_", device)
     ct = _float_type(out_dtype, "out_dtype")
     if c is None:
-        c = w_codes.new_empty((m_tokens, n_rows), dtype=out_dtype)
+        c = torch.empty(m_tokens, n_rows, dtype=out_dtype, device=w_codes.device)
     cp = _ptr(c, out_dtype, "c", m_tokens * n_rows, device)
-    _launch(device, _ffi.lib().axc_cuda_mxfp4_prefill, wp, wsp, ap, asp, cp, ct, m_tokens, n_rows, n_blocks,
-            (_status_ptr(status, device),))
+    _call(device, _lib().axc_cuda_mxfp4_prefill, wp, wsp, ap, asp, cp, ct, m_tokens, n_rows, n_blocks, _raw_stream(device),
+          _status_ptr(status, device))
     return c
 
 
@@ -303,9 +310,9 @@ def _embed(fn, ptrs, device: int, ids, rows: int, n: int, elems: int, scale, out
     ot = _float_type(out_dtype, "out_dtype")
     ip = _ptr(ids, ids.dtype, "ids", 0, device)
     if out is None:
-        out = ids.new_empty((*ids.shape, n * elems), dtype=out_dtype)
+        out = torch.empty(*ids.shape, n * elems, dtype=out_dtype, device=ids.device)
     op = _ptr(out, out_dtype, "out", n_ids * n * elems, device)
-    _launch(device, fn, *ptrs, ip, it, n_ids, op, ot, rows, n, scale, (_status_ptr(status, device),))
+    _call(device, fn, *ptrs, ip, it, n_ids, op, ot, rows, n, scale, _raw_stream(device), _status_ptr(status, device))
     return out
 
 
@@ -317,7 +324,7 @@ def q4k_embed(q: torch.Tensor, ids: torch.Tensor, rows: int, n_superblocks: int,
     device = _device_of(q, "q")
     rows, n = _count(rows, "rows"), _count(n_superblocks, "n_superblocks")
     qp = _ptr(q, torch.uint8, "q", rows * n * Q4K_SB_BYTES, device)
-    return _embed(_ffi.lib().axc_cuda_q4k_embed, (qp,), device, ids, rows, n, Q4K_SB_ELEMS, scale, out, out_dtype, status)
+    return _embed(_lib().axc_cuda_q4k_embed, (qp,), device, ids, rows, n, Q4K_SB_ELEMS, scale, out, out_dtype, status)
 
 
 def q4_0_embed(q: torch.Tensor, ids: torch.Tensor, rows: int, n_blocks: int, scale: float = 1.0,
@@ -327,7 +334,7 @@ def q4_0_embed(q: torch.Tensor, ids: torch.Tensor, rows: int, n_blocks: int, sca
     device = _device_of(q, "q")
     rows, n = _count(rows, "rows"), _count(n_blocks, "n_blocks")
     qp = _ptr(q, torch.uint8, "q", rows * n * Q4_0_BLK_BYTES, device)
-    return _embed(_ffi.lib().axc_cuda_q4_0_embed, (qp,), device, ids, rows, n, Q4_0_BLK_ELEMS, scale, out, out_dtype, status)
+    return _embed(_lib().axc_cuda_q4_0_embed, (qp,), device, ids, rows, n, Q4_0_BLK_ELEMS, scale, out, out_dtype, status)
 
 
 def mxfp4_embed(codes: torch.Tensor, scales: torch.Tensor, ids: torch.Tensor, rows: int, n_blocks: int, scale: float = 1.0,
@@ -336,5 +343,5 @@ def mxfp4_embed(codes: torch.Tensor, scales: torch.Tensor, ids: torch.Tensor, ro
     """``q4k_embed`` for an MXFP4 matrix."""
     device = _device_of(codes, "codes")
     rows, n = _count(rows, "rows"), _count(n_blocks, "n_blocks")
-    return _embed(_ffi.lib().axc_cuda_mxfp4_embed, _mx_operand(codes, scales, rows, n, "", device), device, ids, rows, n,
+    return _embed(_lib().axc_cuda_mxfp4_embed, _mx_operand(codes, scales, rows, n, "", device), device, ids, rows, n,
                   MX_BLOCK_ELEMS, scale, out, out_dtype, status)
