@@ -1,11 +1,13 @@
 // C[m][n] = sum_k A[m][k] W[n][k] for many tokens, A and W in MXFP4: the form of axc_cuda_mxfp4_prefill that is
 // bound by the tensor cores (tcgen05.mma kind::mxf4, block scales, fp32 accumulators in tensor memory).
 //
-// A pair of CTAs (a cluster of two) computes tiles of 256 weight rows (the MMA's M, 128 TMEM lanes in each CTA) x 256
-// tokens (its N, 256 TMEM columns) with tcgen05.mma.cta_group::2: each CTA holds its own 128 weight rows and one half
-// of the tokens, so that per SM 32 KB of codes feed 128 x 256 x 256 products.  One CTA alone would have to read 48 KB
-// through the same shared-memory port.  The pairs are persistent and take tiles in a fixed order, tokens first, so
-// that the pairs at work share the weights through L2.
+// A pair of CTAs (a cluster of two) computes pieces of 256 weight rows (the MMA's M, 128 TMEM lanes in each CTA) x up to
+// 256 tokens (its N, as many TMEM columns) with tcgen05.mma.cta_group::2: each CTA holds its own 128 weight rows and one
+// half of the tokens, so that per SM 32 KB of codes feed 128 x 256 x 256 products.  One CTA alone would have to read 48 KB
+// through the same shared-memory port.  The pairs are persistent and take the
+// pieces in turn, tokens first, so that the pairs at work share the weights through L2.  (Equal contiguous parts for the
+// pairs, cut at 128 tokens, were measured and are not used: 768 x 9472 x 4096 17.9 us either way, 4096 x 28672 x 8192 329 us
+// against 442 us, where every pair reads weights of its own.)
 //
 //   warp 0       one thread: TMA loads of this CTA's codes (128-byte swizzle, stages of 256 columns) and bulk copies
 //                of the scale tiles of its rows and of all 256 tokens
@@ -15,9 +17,8 @@
 //   warps 2..9   epilogue: 128 of the 256 columns each to registers, tensor memory is free again, then the stores,
 //                while the next tile's MMAs run
 //
-// The accumulators are never split: a chain of K / 64 MMAs truncates, which costs up to 1.2e-7 * K / 512 of the value
-// (measured; nothing while all partial sums are multiples of one unit below 2^24).  Callers with fp32 output whose
-// rows are longer than GEMM_CHAIN_BLOCKS go to the split form (mxfp4_product.cu).
+// The accumulators truncate: measured, a chain of K / 64 MMAs loses up to 1.2e-7 * K / 512 of its value when the scales of
+// a row are far apart, and nothing while all partial sums are multiples of one unit below 2^24.
 //
 // Every wait on an mbarrier is bounded; a wait that runs out sets an error bit and an abort flag, all roles fall
 // through to the common exit, outstanding copies are waited for and tensor memory is freed.
@@ -30,7 +31,7 @@
 namespace axc {
 namespace {
 
-constexpr uint32_t GM_ROWS = 256, GM_TOKENS = 256;     // tile of a pair
+constexpr uint32_t GM_ROWS = 256, GM_TOKENS = 256;     // largest piece of a pair
 constexpr uint32_t GM_STAGES = 6;
 constexpr uint32_t GM_W_BYTES = 128 * 128, GM_A_BYTES = 128 * 128;       // codes of a stage in one CTA
 constexpr uint32_t GM_SFW_BYTES = 1024, GM_SFA_BYTES = 2048;
@@ -50,7 +51,7 @@ struct GmArgs {
     const uint8_t* a_scales;
     void* c;
     uint32_t m, rows, n_blocks;
-    uint32_t token_tiles, tiles;
+    uint32_t token_pieces, pieces;   // pieces of 256 tokens per row tile and in all
     uint32_t* status;
 };
 
@@ -74,6 +75,22 @@ __device__ __forceinline__ void umma_mxf4_pair(uint32_t d, uint64_t a_desc, uint
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
         : "memory");
 }
+
+// The pieces of one pair, in order.
+struct Pieces {
+    uint32_t at, end, step, per_row, m;
+    uint32_t row_tile, tok0, n;   // n: columns of the MMA, the tokens rounded up to 32
+    __device__ __forceinline__ Pieces(const GmArgs& p, uint32_t pair, uint32_t pairs)
+        : at(pair), end(p.pieces), step(pairs), per_row(p.token_pieces), m(p.m) {}
+    __device__ __forceinline__ bool next() {
+        if (at >= end) return false;
+        row_tile = at / per_row;
+        tok0 = (at - row_tile * per_row) * GM_TOKENS;
+        n = (min(GM_TOKENS, m - tok0) + 31u) & ~31u;
+        at += step;
+        return true;
+    }
+};
 
 template <typename Out>
 __global__ void __launch_bounds__(GM_THREADS, 1)
@@ -117,9 +134,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
         // The whole warp runs the loop, an elected lane issues.
         uint32_t issued = 0, s = 0, ph = 1;
         bool ok = true;
-        for (uint32_t tile = pair; tile < p.tiles && ok; tile += pairs) {
-            const uint32_t row0 = tile / p.token_tiles * GM_ROWS + rank * 128u, tok0 = tile % p.token_tiles * GM_TOKENS;
-            // scale tiles that exist: the last pair may have no rows in its second CTA, the last tokens one tile
+        Pieces it(p, pair, pairs);
+        while (ok && it.next()) {
+            const uint32_t row0 = it.row_tile * GM_ROWS + rank * 128u, tok0 = it.tok0;
+            // scale tiles that exist: the last row tile may have no rows for the second CTA, the last tokens one tile
             const bool has_rows = row0 / 128u < row_tiles;
             const uint32_t a_tiles = min(2u, tok_tiles - tok0 / 128u);
             const uint8_t* sw = p.w_scales + (uint64_t)(row0 / 128u) * n_quads * MX_TILE_BYTES;
@@ -132,8 +150,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
                     uint8_t* stage = sm + s * GM_STAGE_BYTES;
                     mbar_expect_tx(&bars->full[s], GM_W_BYTES + GM_A_BYTES + ((has_rows ? 1u : 0u) + a_tiles) * quad_bytes);
                     tma_load_2d(base + s * GM_STAGE_BYTES, &tm_w, (int32_t)(st * 128u), (int32_t)row0, &bars->full[s]);
-                    tma_load_2d(base + s * GM_STAGE_BYTES + GM_OFF_A, &tm_a, (int32_t)(st * 128u), (int32_t)(tok0 + rank * 128u),
-                                &bars->full[s]);
+                    tma_load_2d(base + s * GM_STAGE_BYTES + GM_OFF_A, &tm_a, (int32_t)(st * 128u), (int32_t)(tok0 + rank * (it.n / 2u)),
+                                &bars->full[s]);   // a whole box; the MMA takes the first half of the piece's tokens
                     if (has_rows) bulk_g2s(stage + GM_OFF_SFW, sw + st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
                     bulk_g2s(stage + GM_OFF_SFA, sa + st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
                     if (a_tiles > 1u)
@@ -151,8 +169,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
         if (leader) {
             bool ok = true;
             uint32_t s = 0, ph = 0, acc_ph = 1;
-            if (elect_one()) for (uint32_t tile = pair; tile < p.tiles && ok; tile += pairs, acc_ph ^= 1u) {
-                ok = mbar_wait_or_abort(&bars->acc_empty, acc_ph, &bars->abort, p.status);   // the last tile is read
+            Pieces it(p, pair, pairs);
+            if (elect_one()) for (; ok && it.next(); acc_ph ^= 1u) {
+                const uint32_t idesc = mx_idesc(256u, it.n, 0u), idesc2 = mx_idesc(256u, it.n, 2u);
+                ok = mbar_wait_or_abort(&bars->acc_empty, acc_ph, &bars->abort, p.status);   // the last piece is read
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (uint32_t st = 0; st < n_st; ++st) {
@@ -173,7 +193,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
 #pragma unroll
                         for (uint32_t kk = 0; kk < 4u; ++kk) {
                             if (kk >= steps) break;
-                            umma_mxf4_pair(0u, wd + 2u * kk, ad + 2u * kk, mx_idesc(256u, GM_TOKENS, (kk & 1u) * 2u),
+                            umma_mxf4_pair(0u, wd + 2u * kk, ad + 2u * kk, kk & 1u ? idesc2 : idesc,
                                            sf + (kk >> 1) * 4u, sf + 8u + (kk >> 1) * 8u, (st | kk) != 0u);
                         }
                         umma_commit_pair(&bars->empty[s]);
@@ -184,30 +204,32 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
             }
         } else if (lane == 0) {
             // peer: tell the leader when this CTA's stage has landed
-            uint32_t it = 0;
-            for (uint32_t tile = pair; tile < p.tiles && !bars->abort; tile += pairs)
-                for (uint32_t st = 0; st < n_st && !bars->abort; ++st, ++it) {
-                    if (!mbar_wait(&bars->full[it % GM_STAGES], (it / GM_STAGES) & 1u, p.status)) {
-                        bars->abort = 1;
-                        break;
-                    }
-                    mbar_arrive_remote(&bars->full[it % GM_STAGES], 0u);
+            uint32_t s = 0, ph = 0;
+            bool ok = true;
+            Pieces it(p, pair, pairs);
+            while (ok && it.next())
+                for (uint32_t st = 0; st < n_st; ++st) {
+                    ok = mbar_wait_or_abort(&bars->full[s], ph, &bars->abort, p.status);
+                    if (!ok) break;
+                    mbar_arrive_remote(&bars->full[s], 0u);
+                    if (++s == GM_STAGES) s = 0, ph ^= 1u;
                 }
         }
     } else {
         // ---------------- epilogue: TMEM lane = weight row, column = token ----------------
-        const uint32_t quad = warp & 3u, half = (warp - 2u) >> 2;   // warps 2..5: tokens 0..127, warps 6..9: 128..255
-        uint32_t done = 0;
+        const uint32_t quad = warp & 3u, half = (warp - 2u) >> 2;   // warps 2..5: the first half of the tokens, 6..9: the second
+        uint32_t ph = 0;
         bool ok = true;
-        for (uint32_t tile = pair; tile < p.tiles && ok; tile += pairs, ++done) {
-            const uint32_t row = tile / p.token_tiles * GM_ROWS + rank * 128u + quad * 32u + lane;
-            const uint32_t tok0 = tile % p.token_tiles * GM_TOKENS + half * 128u;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bars->acc_full, done & 1u, p.status) && !bars->abort);
+        for (Pieces it(p, pair, pairs); ok && it.next(); ph ^= 1u) {
+            const uint32_t row = it.row_tile * GM_ROWS + rank * 128u + quad * 32u + lane;
+            const uint32_t col0 = half * (it.n / 2u), tok0 = it.tok0 + col0;
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->acc_full, ph, &bars->abort, p.status));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            uint32_t v[4][32];
+            uint32_t v[8][16];
 #pragma unroll
-            for (uint32_t b = 0; b < 4u; ++b) tmem_load32(tmem + ((quad * 32u) << 16) + half * 128u + b * 32u, v[b]);
+            for (uint32_t b = 0; b < 8u; ++b)
+                if (b * 32u < it.n) tmem_load16(tmem + ((quad * 32u) << 16) + col0 + b * 16u, v[b]);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -216,21 +238,20 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
                 else mbar_arrive_remote(&bars->acc_empty, 0u);
             }
             if (row < p.rows && tok0 < p.m) {
-                // a whole tile without a test per value: with tests a warp took 10 000 cycles here instead of the
-                // 2 000 that fit behind the next tile's MMAs (2048 x 18944 x 4096: 68 us)
+                // sixteen tokens without a test per value: with tests a warp took 10 000 cycles here instead of the
+                // 3 400 that fit behind the next piece's MMAs (2048 x 18944 x 4096: 68 us)
                 Out* dst = reinterpret_cast<Out*>(p.c) + (uint64_t)tok0 * p.rows + row;
-                const uint32_t count = p.m - tok0;
-                if (count >= 128u) {
+                const uint32_t count = min(p.m - tok0, it.n / 2u);
 #pragma unroll
-                    for (uint32_t b = 0; b < 4u; ++b)
+                for (uint32_t b = 0; b < 8u; ++b) {
+                    if (b * 16u + 16u <= count) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 32u; ++j, dst += p.rows) put(dst, __uint_as_float(v[b][j]));
-                } else {
+                        for (uint32_t j = 0; j < 16u; ++j, dst += p.rows) put(dst, __uint_as_float(v[b][j]));
+                    } else {
 #pragma unroll
-                    for (uint32_t b = 0; b < 4u; ++b)
-#pragma unroll
-                        for (uint32_t j = 0; j < 32u; ++j, dst += p.rows)
-                            if (b * 32u + j < count) put(dst, __uint_as_float(v[b][j]));
+                        for (uint32_t j = 0; j < 16u; ++j, dst += p.rows)
+                            if (b * 16u + j < count) put(dst, __uint_as_float(v[b][j]));
+                    }
                 }
             }
         }
@@ -277,7 +298,7 @@ cudaError_t launch(const CUtensorMap& tm_w, const CUtensorMap& tm_a, const GmArg
             pairs = fits[dev];
         }
     }
-    cfg.gridDim = dim3(2u * (p.tiles < (uint32_t)pairs ? p.tiles : (uint32_t)pairs)), cfg.numAttrs = 2;
+    cfg.gridDim = dim3(2u * (p.pieces < (uint32_t)pairs ? p.pieces : (uint32_t)pairs)), cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kern, tm_w, tm_a, p);
 }
 
@@ -290,8 +311,10 @@ cudaError_t launch_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, c
     CUtensorMap tm_w, tm_a;
     if (!mx_encode_codes(&tm_w, w_codes, n_rows, n_blocks, 128u) || !mx_encode_codes(&tm_a, a_codes, m_tokens, n_blocks, 128u))
         return cudaErrorInvalidValue;
-    GmArgs p{w_scales, a_scales, c, m_tokens, n_rows, n_blocks, (m_tokens + GM_TOKENS - 1u) / GM_TOKENS, 0, status};
-    p.tiles = (n_rows + GM_ROWS - 1u) / GM_ROWS * p.token_tiles;
+    const uint32_t token_pieces = (m_tokens + GM_TOKENS - 1u) / GM_TOKENS;
+    const uint64_t pieces = (uint64_t)((n_rows + GM_ROWS - 1u) / GM_ROWS) * token_pieces;
+    if (pieces >= 1u << 31) return cudaErrorInvalidConfiguration;
+    const GmArgs p{w_scales, a_scales, c, m_tokens, n_rows, n_blocks, token_pieces, (uint32_t)pieces, status};
     switch (type) {
         case ElemType::F32: return launch<float>(tm_w, tm_a, p, stream, sm_count);
         case ElemType::BF16: return launch<__nv_bfloat16>(tm_w, tm_a, p, stream, sm_count);

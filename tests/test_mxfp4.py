@@ -209,7 +209,8 @@ def check_prefill(ops, m, n, nb, dtype, seed, low=118, high=124):
 
 @gpu
 @pytest.mark.parametrize("m,n,nb", [(1, 1, 1), (1, 128, 2), (5, 300, 7), (16, 128, 8), (17, 130, 3), (37, 513, 33), (64, 96, 128),
-                                    (128, 128, 16), (256, 256, 8), (257, 129, 9), (300, 200, 4), (513, 384, 11), (600, 640, 5)])
+                                    (128, 128, 16), (256, 256, 8), (257, 129, 9), (300, 200, 4), (513, 384, 11), (600, 640, 5),
+                                    (520, 3000, 6), (1000, 2310, 10), (80, 19200, 5), (128, 700, 40)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_prefill_matches_float64(ops, m, n, nb, dtype):
     check_prefill(ops, m, n, nb, dtype, m * 1000 + n + nb)
