@@ -216,9 +216,12 @@ def _tile_bytes(rows: int, n_blocks: int) -> int:
     return (rows + 127) // 128 * ((n_blocks + 3) // 4) * 512
 
 
-def _mx_operand(codes, scales, rows: int, n_blocks: int, name: str, device: int):
-    return (_ptr(codes, torch.uint8, name + "codes", rows * n_blocks * MX_BLOCK_BYTES, device),
-            _ptr(scales, torch.uint8, name + "scales", _tile_bytes(rows, n_blocks), device))
+def _codes_ptr(codes, rows: int, n_blocks: int, device: int, name: str = "codes") -> int:
+    return _ptr(codes, torch.uint8, name, rows * n_blocks * MX_BLOCK_BYTES, device)
+
+
+def _scales_ptr(scales, rows: int, n_blocks: int, device: int, name: str = "scales") -> int:
+    return _ptr(scales, torch.uint8, name, _tile_bytes(rows, n_blocks), device)
 
 
 def mxfp4_quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None):
@@ -244,9 +247,14 @@ def mxfp4_quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales
     n_blocks = (cols + 31) // 32
     if codes is None:
         codes = torch.empty(rows, n_blocks * MX_BLOCK_BYTES, dtype=torch.uint8, device=x.device)
+        cp = codes.data_ptr()
+    else:
+        cp = _codes_ptr(codes, rows, n_blocks, device)
     if scales is None:
         scales = torch.empty(_tile_bytes(rows, n_blocks), dtype=torch.uint8, device=x.device)
-    cp, sp = _mx_operand(codes, scales, rows, n_blocks, "", device)
+        sp = scales.data_ptr()
+    else:
+        sp = _scales_ptr(scales, rows, n_blocks, device)
     _call(device, _lib().axc_cuda_mxfp4_quantize, x.data_ptr(), xt, stride, rows, cols, cp, sp, _raw_stream(device))
     return codes, scales
 
@@ -257,11 +265,13 @@ def mxfp4_dequant(codes: torch.Tensor, scales: torch.Tensor, rows: int, n_blocks
     bfloat16 / float16."""
     device = _device_of(codes, "codes")
     rows, n_blocks = _count(rows, "rows"), _count(n_blocks, "n_blocks")
-    cp, sp = _mx_operand(codes, scales, rows, n_blocks, "", device)
+    cp, sp = _codes_ptr(codes, rows, n_blocks, device), _scales_ptr(scales, rows, n_blocks, device)
     wt = _float_type(out_dtype, "out_dtype")
     if w is None:
         w = torch.empty(rows, n_blocks * MX_BLOCK_ELEMS, dtype=out_dtype, device=codes.device)
-    wp = _ptr(w, out_dtype, "w", rows * n_blocks * MX_BLOCK_ELEMS, device)
+        wp = w.data_ptr()
+    else:
+        wp = _ptr(w, out_dtype, "w", rows * n_blocks * MX_BLOCK_ELEMS, device)
     _call(device, _lib().axc_cuda_mxfp4_dequant, cp, sp, wp, wt, rows, n_blocks, _raw_stream(device))
     return w
 
@@ -273,12 +283,14 @@ def mxfp4_matvec(codes: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, row
     dimensions than one or there are several."""
     device = _device_of(codes, "codes")
     rows, n_blocks, m_tokens = _count(rows, "rows"), _count(n_blocks, "n_blocks"), _count(m_tokens, "m_tokens", 1)
-    cp, sp = _mx_operand(codes, scales, rows, n_blocks, "", device)
+    cp, sp = _codes_ptr(codes, rows, n_blocks, device), _scales_ptr(scales, rows, n_blocks, device)
     xp = _ptr(x, torch.float32, "x", m_tokens * n_blocks * MX_BLOCK_ELEMS, device)
     if y is None:
         y = torch.empty(rows, dtype=torch.float32, device=x.device) if m_tokens == 1 and x.dim() <= 1 else \
             torch.empty(m_tokens, rows, dtype=torch.float32, device=x.device)
-    yp = _ptr(y, torch.float32, "y", m_tokens * rows, device)
+        yp = y.data_ptr()
+    else:
+        yp = _ptr(y, torch.float32, "y", m_tokens * rows, device)
     _call(device, _lib().axc_cuda_mxfp4_matvec, cp, sp, xp, yp, m_tokens, rows, n_blocks, _raw_stream(device),
           _status_ptr(status, device))
     return y
@@ -291,12 +303,14 @@ def mxfp4_prefill(w_codes: torch.Tensor, w_scales: torch.Tensor, a_codes: torch.
     ``mxfp4_quantize``): C has shape (m_tokens, n_rows) in out_dtype, fp32 accumulation, one rounding."""
     device = _device_of(w_codes, "w_codes")
     m_tokens, n_rows, n_blocks = _count(m_tokens, "m_tokens"), _count(n_rows, "n_rows"), _count(n_blocks, "n_blocks")
-    wp, wsp = _mx_operand(w_codes, w_scales, n_rows, n_blocks, "w_", device)
-    ap, asp = _mx_operand(a_codes, a_scales, m_tokens, n_blocks, "a_", device)
+    wp, wsp = _codes_ptr(w_codes, n_rows, n_blocks, device, "w_codes"), _scales_ptr(w_scales, n_rows, n_blocks, device, "w_scales")
+    ap, asp = _codes_ptr(a_codes, m_tokens, n_blocks, device, "a_codes"), _scales_ptr(a_scales, m_tokens, n_blocks, device, "a_scales")
     ct = _float_type(out_dtype, "out_dtype")
     if c is None:
         c = torch.empty(m_tokens, n_rows, dtype=out_dtype, device=w_codes.device)
-    cp = _ptr(c, out_dtype, "c", m_tokens * n_rows, device)
+        cp = c.data_ptr()
+    else:
+        cp = _ptr(c, out_dtype, "c", m_tokens * n_rows, device)
     _call(device, _lib().axc_cuda_mxfp4_prefill, wp, wsp, ap, asp, cp, ct, m_tokens, n_rows, n_blocks, _raw_stream(device),
           _status_ptr(status, device))
     return c
@@ -311,7 +325,9 @@ def _embed(fn, ptrs, device: int, ids, rows: int, n: int, elems: int, scale, out
     ip = _ptr(ids, ids.dtype, "ids", 0, device)
     if out is None:
         out = torch.empty(*ids.shape, n * elems, dtype=out_dtype, device=ids.device)
-    op = _ptr(out, out_dtype, "out", n_ids * n * elems, device)
+        op = out.data_ptr()
+    else:
+        op = _ptr(out, out_dtype, "out", n_ids * n * elems, device)
     _call(device, fn, *ptrs, ip, it, n_ids, op, ot, rows, n, scale, _raw_stream(device), _status_ptr(status, device))
     return out
 
@@ -343,5 +359,5 @@ def mxfp4_embed(codes: torch.Tensor, scales: torch.Tensor, ids: torch.Tensor, ro
     """``q4k_embed`` for an MXFP4 matrix."""
     device = _device_of(codes, "codes")
     rows, n = _count(rows, "rows"), _count(n_blocks, "n_blocks")
-    return _embed(_lib().axc_cuda_mxfp4_embed, _mx_operand(codes, scales, rows, n, "", device), device, ids, rows, n,
-                  MX_BLOCK_ELEMS, scale, out, out_dtype, status)
+    ptrs = _codes_ptr(codes, rows, n, device), _scales_ptr(scales, rows, n, device)
+    return _embed(_lib().axc_cuda_mxfp4_embed, ptrs, device, ids, rows, n, MX_BLOCK_ELEMS, scale, out, out_dtype, status)
