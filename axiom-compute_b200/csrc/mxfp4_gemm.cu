@@ -157,8 +157,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
                     tma_load_2d(base + s * GM_STAGE_BYTES, &tm_w, (int32_t)(st * 128u), (int32_t)row0, &bars->full[s]);
                     tma_load_2d(base + s * GM_STAGE_BYTES + GM_OFF_A, &tm_a, (int32_t)(st * 128u), (int32_t)(tok0 + rank * (it.n / 2u)),
                                 &bars->full[s]);   // a whole box; the MMA takes the first half of the piece's tokens
-                    if (has_rows) bulk_g2s(stage + GM_OFF_SFW, sw + st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
-                    bulk_g2s(stage + GM_OFF_SFA, sa + st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
+                    if (has_rows) bulk_g2s(stage + GM_OFF_SFW, sw + (uint64_t)st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
+                    bulk_g2s(stage + GM_OFF_SFA, sa + (uint64_t)st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
                     if (a_tiles > 1u)
                         bulk_g2s(stage + GM_OFF_SFA + 1024u, sa + ((uint64_t)n_quads + st * 2u) * MX_TILE_BYTES, quad_bytes,
                                  &bars->full[s]);

@@ -337,8 +337,8 @@ int axc_cuda_mxfp4_dequant(const void* codes, const void* scales, void* w, uint3
  * block's largest |x| (error at most 2^-22 of that), and the products with its base-8 digits are exact on the tensor
  * cores; sums are fp32.  Blocks whose largest |x| is below 2^-105 keep the absolute resolution
  * 2^-127.  A block of x with a NaN, an infinity or a magnitude of 2^127 or more makes every y of that token NaN.
- * n_blocks = 0 gives zeros.  *status (nullable) receives bit 0
- * if a bounded wait inside the kernel ran out. */
+ * n_blocks = 0 gives zeros.  A token's y has the same bits whatever other tokens the call serves.  *status (nullable)
+ * receives bit 0 if a bounded wait inside the kernel ran out. */
 #define AXC_MXFP4_MATVEC_TOKENS 8
 int axc_cuda_mxfp4_matvec(const void* codes, const void* scales, const float* x, float* y, uint32_t m_tokens, uint32_t rows,
                           uint32_t n_blocks, void* stream, uint32_t* status);

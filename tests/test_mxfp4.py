@@ -1,9 +1,13 @@
 """MXFP4: quantisation, dequantisation, the fp32 matvec and the block-scaled product against a float64 restatement of
 the format, and their refusals."""
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
 
+from conftest import ROOT
 from oracle import mxfp4_np as mx
 
 gpu = pytest.mark.gpu
@@ -353,6 +357,73 @@ def test_zero_sizes(ops):
     assert ops.mxfp4_prefill(torch.zeros(5 * 48, dtype=torch.uint8, device="cuda"), torch.zeros(512, dtype=torch.uint8, device="cuda"),
                              e, e, 0, 5, 3).shape == (0, 5)
     assert int(st.item()) == 0
+
+
+def large_operands(ops, rows, nb, seed, spread=0.02):
+    """A matrix quantised on the device and its values (exact in fp32) as float64."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes, scales = ops.mxfp4_quantize(torch.randn(rows, nb * 32, generator=g, device="cuda") * spread)
+    return codes, scales, ops.mxfp4_dequant(codes, scales, rows, nb).double()
+
+
+@gpu
+@pytest.mark.parametrize("rows,nb", [(1100, 600), (9000, 200), (4096, 128), (14336, 40), (40000, 16), (700, 1000), (129, 2100),
+                                     (20000, 30), (1024, 25), (1024, 24)])
+def test_matvec_over_the_forms_of_the_kernel(ops, rows, nb):
+    """One and two row tiles, 1 to 8 CTAs per row, rings that wrap, every number of tokens."""
+    codes, scales, w = large_operands(ops, rows, nb, rows + nb)
+    x = torch.randn(8, nb * 32, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    x64 = x.double()
+    ref, mag = x64 @ w.t(), x64.abs() @ w.abs().t()
+    top = x64.abs().view(8, nb, 32).amax(dim=2).repeat_interleave(32, dim=1)
+    fixed = 2.0 ** -22 * (top @ w.abs().t())
+    all8 = ops.mxfp4_matvec(codes, scales, x, rows, nb, m_tokens=8)
+    assert bool(((all8.double() - ref).abs() <= fixed + chain_bound(nb) * (4 * mag + 8 * fixed)).all())
+    for m in range(1, 8):                                 # the same bits whatever other tokens the call serves
+        st = ops.new_status()
+        assert torch.equal(ops.mxfp4_matvec(codes, scales, x[8 - m:], rows, nb, m_tokens=m, status=st), all8[8 - m:]), m
+        assert int(st.item()) == 0
+
+
+@gpu
+@pytest.mark.parametrize("m,n,nb", [(40, 1100, 600), (64, 9000, 200), (33, 25000, 16), (64, 20000, 50), (100, 3000, 300), (128, 1000, 900),
+                                    (128, 19500, 20), (65, 9600, 40), (129, 4000, 130), (1000, 5000, 100), (2048, 9500, 24),
+                                    (3, 60000, 9)])
+def test_prefill_over_the_forms_of_the_kernels(ops, m, n, nb):
+    w_codes, w_scales, w = large_operands(ops, n, nb, n + nb)
+    a_codes, a_scales, a = large_operands(ops, m, nb, m + nb, 3.0)
+    st = ops.new_status()
+    c = ops.mxfp4_prefill(w_codes, w_scales, a_codes, a_scales, m, n, nb, status=st)
+    assert int(st.item()) == 0
+    assert bool(((c.double() - a @ w.t()).abs() <= chain_bound(nb) * (a.abs() @ w.abs().t())).all())
+    for dtype in (torch.bfloat16, torch.float16):         # the same sums, rounded once
+        assert torch.equal(ops.mxfp4_prefill(w_codes, w_scales, a_codes, a_scales, m, n, nb, out_dtype=dtype), c.to(dtype))
+
+
+@gpu
+def test_first_call_may_be_captured():
+    """In a process that has not used the library yet, every call goes into a graph at once."""
+    code = """
+import importlib, torch
+ops = importlib.import_module("axiom-compute_b200.ops")
+x = torch.randn(300, 640, device="cuda"); w = torch.randn(1100, 640, device="cuda"); ids = torch.arange(5, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    wc, ws = ops.mxfp4_quantize(w)
+    xc, xs = ops.mxfp4_quantize(x)
+    c = ops.mxfp4_prefill(wc, ws, xc, xs, 300, 1100, 20)
+    few = ops.mxfp4_prefill(wc, ws, xc, xs, 40, 1100, 20)
+    y = ops.mxfp4_matvec(wc, ws, x[:3], 1100, 20, m_tokens=3)
+    e = ops.mxfp4_embed(wc, ws, ids, 1100, 20)
+    v = ops.mxfp4_dequant(wc, ws, 1100, 20)
+g.replay(); torch.cuda.synchronize()
+assert torch.equal(e, v[:5]) and torch.equal(few, ops.mxfp4_prefill(wc, ws, xc, xs, 40, 1100, 20))
+assert torch.equal(c, ops.mxfp4_prefill(wc, ws, xc, xs, 300, 1100, 20))
+assert torch.equal(y, ops.mxfp4_matvec(wc, ws, x[:3], 1100, 20, m_tokens=3))
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 @gpu
