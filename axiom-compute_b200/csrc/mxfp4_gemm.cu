@@ -11,14 +11,11 @@
 //
 //   warp 0       one thread: TMA loads of this CTA's codes (128-byte swizzle, stages of 256 columns) and bulk copies
 //                of the scale tiles of its rows and of all 256 tokens
-//   warp 1       leader: one thread issues four MMAs of 64 columns per stage and the commit that frees the stage in both
-//                CTAs; it looks at the next stage's barriers before the MMAs of this one, so that a stage costs it less
-//                than the 512 cycles of its MMAs
-//   warp 2       leader: one thread copies the stage's scales into both CTAs' tensor memory (tcgen05.cp; in the MMA
-//                thread these took 220 of 620 cycles per stage); peer: one thread tells the leader when its stage has
-//                landed
-//   warps 3..10  epilogue: 128 of the 256 columns each to registers, tensor memory is free again, then the stores,
-//                while the next piece's MMAs run
+//   warp 1       leader: one thread copies the stage's scales into both CTAs' tensor memory (tcgen05.cp), issues four
+//                MMAs of 64 columns and the commit that frees the stage in both CTAs; peer: one thread tells the
+//                leader when its stage has landed
+//   warps 2..9   epilogue: 128 of the 256 columns each to registers, tensor memory is free again, then the stores,
+//                while the next tile's MMAs run
 //
 // The accumulators truncate: measured, a chain of K / 64 MMAs loses up to 1.2e-7 * K / 512 of its value when the scales of
 // a row are far apart, and nothing while all partial sums are multiples of one unit below 2^24.
@@ -43,8 +40,7 @@ constexpr uint32_t GM_OFF_A = GM_W_BYTES, GM_OFF_SFW = GM_OFF_A + GM_A_BYTES, GM
 constexpr uint32_t GM_OFF_BAR = GM_STAGES * GM_STAGE_BYTES;
 constexpr uint32_t GM_SMEM = GM_OFF_BAR + 256 + 1024;                     // + alignment slack
 constexpr uint32_t GM_EPI_WARPS = 8;
-constexpr uint32_t GM_FIRST_EPI = 3;
-constexpr uint32_t GM_THREADS = (GM_FIRST_EPI + GM_EPI_WARPS) * 32;
+constexpr uint32_t GM_THREADS = (2 + GM_EPI_WARPS) * 32;
 constexpr uint32_t GM_SF_COL = 256;                    // scale columns behind the accumulator: 24 for each stage
 static_assert(GM_STAGE_BYTES % 1024 == 0, "the swizzled tiles need 1024-byte alignment");
 static_assert(GM_SF_COL + GM_STAGES * 24 <= 512, "tensor memory");
@@ -61,7 +57,6 @@ struct GmArgs {
 
 struct GmBars {
     uint64_t full[GM_STAGES], empty[GM_STAGES];
-    uint64_t scaled[GM_STAGES];   // the stage's scales are in tensor memory
     uint64_t acc_full, acc_empty;
     uint32_t tmem_base;
     volatile uint32_t abort;
@@ -115,7 +110,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
     const uint32_t row_tiles = (p.rows + 127u) / 128u, tok_tiles = (p.m + 127u) / 128u;   // scale tiles of W and A
 
     if (tid == 0) {
-        for (uint32_t s = 0; s < GM_STAGES; ++s) mbar_init(&bars->full[s], leader ? 2u : 1u), mbar_init(&bars->empty[s], 1), mbar_init(&bars->scaled[s], 1);
+        for (uint32_t s = 0; s < GM_STAGES; ++s) mbar_init(&bars->full[s], leader ? 2u : 1u), mbar_init(&bars->empty[s], 1);
         mbar_init(&bars->acc_full, 1);
         mbar_init(&bars->acc_empty, leader ? 2u * GM_EPI_WARPS : 1u);
         bars->abort = 0;
@@ -171,68 +166,58 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
         for (uint32_t j = issued > GM_STAGES ? issued - GM_STAGES : 0; j < issued; ++j)
             (void)mbar_wait(&bars->full[j % GM_STAGES], (j / GM_STAGES) & 1u, p.status);
     } else if (warp == 1) {
-        if (leader && elect_one()) {
-            uint32_t s = 0, ph = 0, acc_ph = 1;
-            uint32_t ready = 0;
+        if (leader) {
             bool ok = true;
-            for (Pieces it(p, pair, pairs); ok && it.next(); acc_ph ^= 1u) {
+            uint32_t s = 0, ph = 0, acc_ph = 1;
+            Pieces it(p, pair, pairs);
+            if (elect_one()) for (; ok && it.next(); acc_ph ^= 1u) {
                 const uint32_t idesc = mx_idesc(256u, it.n, 0u), idesc2 = mx_idesc(256u, it.n, 2u);
                 ok = mbar_wait_or_abort(&bars->acc_empty, acc_ph, &bars->abort, p.status);   // the last piece is read
                 if (!ok) break;
-                for (uint32_t st = 0; st < n_st; ++st) {
-                    if (!ready) {
-                        ok = mbar_wait_or_abort(&bars->full[s], ph, &bars->abort, p.status) &&
-                             mbar_wait_or_abort(&bars->scaled[s], ph, &bars->abort, p.status);
-                        if (!ok) break;
-                    }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t next = s + 1u == GM_STAGES ? 0u : s + 1u, next_ph = next ? ph : ph ^ 1u;
-                    const uint32_t full = mbar_test(&bars->full[next], next_ph), scaled = mbar_test(&bars->scaled[next], next_ph);
-                    const uint32_t steps = min(4u, (p.n_blocks - st * 8u + 1u) / 2u);
-                    const uint32_t sf = GM_SF_COL + s * 24u, stage = base + s * GM_STAGE_BYTES;
-                    const uint64_t wd = sw128_desc(stage), ad = sw128_desc(stage + GM_OFF_A);
-#pragma unroll
-                    for (uint32_t kk = 0; kk < 4u; ++kk) {
-                        if (kk >= steps) break;
-                        umma_mxf4_pair(0u, wd + 2u * kk, ad + 2u * kk, kk & 1u ? idesc2 : idesc, sf + (kk >> 1) * 4u,
-                                       sf + 8u + (kk >> 1) * 8u, (st | kk) != 0u);
-                    }
-                    umma_commit_pair(&bars->empty[s]);
-                    if (st + 1u == n_st) umma_commit_pair(&bars->acc_full);
-                    ready = full & scaled;
-                    s = next, ph = next_ph;
-                }
-            }
-        }
-    } else if (warp == 2) {
-        if (elect_one()) {
-            uint32_t s = 0, ph = 0;
-            bool ok = true;
-            for (Pieces it(p, pair, pairs); ok && it.next();)
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (uint32_t st = 0; st < n_st; ++st) {
                     ok = mbar_wait_or_abort(&bars->full[s], ph, &bars->abort, p.status);
                     if (!ok) break;
-                    if (leader) {
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t steps = min(4u, (p.n_blocks - st * 8u + 1u) / 2u);
+                    {
                         const uint32_t sf = GM_SF_COL + s * 24u, stage = base + s * GM_STAGE_BYTES;
-                        const uint32_t tiles = min(2u, n_quads - st * 2u);   // scale tiles of this stage
 #pragma unroll
                         for (uint32_t g = 0; g < 2u; ++g) {
-                            if (g >= tiles) break;
+                            if (2u * g >= steps) break;
                             scales_to_tmem_pair(sf + g * 4u, stage + GM_OFF_SFW + g * MX_TILE_BYTES);
                             scales_to_tmem_pair(sf + 8u + g * 8u, stage + GM_OFF_SFA + g * MX_TILE_BYTES);
                             scales_to_tmem_pair(sf + 12u + g * 8u, stage + GM_OFF_SFA + 1024u + g * MX_TILE_BYTES);
                         }
-                        umma_commit_pair(&bars->scaled[s]);
-                    } else {
-                        mbar_arrive_remote(&bars->full[s], 0u);   // tells the leader that this CTA's stage has landed
+                        const uint64_t wd = sw128_desc(stage), ad = sw128_desc(stage + GM_OFF_A);
+#pragma unroll
+                        for (uint32_t kk = 0; kk < 4u; ++kk) {
+                            if (kk >= steps) break;
+                            umma_mxf4_pair(0u, wd + 2u * kk, ad + 2u * kk, kk & 1u ? idesc2 : idesc,
+                                           sf + (kk >> 1) * 4u, sf + 8u + (kk >> 1) * 8u, (st | kk) != 0u);
+                        }
+                        umma_commit_pair(&bars->empty[s]);
+                        if (st + 1u == n_st) umma_commit_pair(&bars->acc_full);
                     }
+                    if (++s == GM_STAGES) s = 0, ph ^= 1u;
+                }
+            }
+        } else if (lane == 0) {
+            // peer: tell the leader when this CTA's stage has landed
+            uint32_t s = 0, ph = 0;
+            bool ok = true;
+            Pieces it(p, pair, pairs);
+            while (ok && it.next())
+                for (uint32_t st = 0; st < n_st; ++st) {
+                    ok = mbar_wait_or_abort(&bars->full[s], ph, &bars->abort, p.status);
+                    if (!ok) break;
+                    mbar_arrive_remote(&bars->full[s], 0u);
                     if (++s == GM_STAGES) s = 0, ph ^= 1u;
                 }
         }
     } else {
         // ---------------- epilogue: TMEM lane = weight row, column = token ----------------
-        const uint32_t quad = warp & 3u, half = (warp - GM_FIRST_EPI) >> 2;   // warps 3..6: the first half of the tokens
+        const uint32_t quad = warp & 3u, half = (warp - 2u) >> 2;   // warps 2..5: the first half of the tokens, 6..9: the second
         uint32_t ph = 0;
         bool ok = true;
         for (Pieces it(p, pair, pairs); ok && it.next(); ph ^= 1u) {

@@ -215,6 +215,7 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     const uint32_t b_stage = p.n * MP_STAGE_BYTES;
     const uint32_t w_tiles = min(TILES, (p.rows + 127u) / 128u - tile0);                 // tiles that exist
 
+    if (p.splits > 1u) cluster_arrive();     // waited for before another CTA's shared memory is written
     if (tid == 0) {
         for (uint32_t s = 0; s < p.stages; ++s) mbar_init(&bars->full[s], 1u + (DIGITS ? p.m : 0u)), mbar_init(&bars->empty[s], 1);
         mbar_init(&bars->done, MP_MMA_WARPS);
@@ -241,7 +242,6 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (p.splits > 1u) cluster_sync_all();   // every CTA of the cluster has started: its shared memory may be written
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = bars->tmem_base;
     asm volatile("griddepcontrol.wait;" ::: "memory");   // an ordered launch: see axc_tuning.pdl
@@ -341,6 +341,7 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         // ---------------- epilogue: TMEM lane = weight row; partial sums to the CTA that finishes the row ----------------
         const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->done, 0u, &bars->abort, p.status));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (p.splits > 1u) cluster_wait();   // every CTA of the cluster has started
         if (ok) {
             // groups of four warps, two for each tile, that take turns at its columns
             const uint32_t t = xw >> 3, grp = (xw >> 2) & 1u, quad = warp & 3u;
@@ -385,7 +386,9 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         }
     }
 
+    __syncwarp();
     if (p.splits > 1u) {
+        if (warp < MP_FIRST_X) cluster_wait();
         cluster_sync_all();
         if (warp >= MP_FIRST_X) {
             const uint32_t per = 1u << p.per_shift, pitch = red_row<DIGITS>(p.m);
