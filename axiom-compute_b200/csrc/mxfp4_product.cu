@@ -339,7 +339,7 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         }
 
         // ---------------- epilogue: TMEM lane = weight row; partial sums to the CTA that finishes the row ----------------
-        const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->done, 0u, &bars->abort, p.status));
+        const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait_or_abort(&bars->done, 0u, &bars->abort, p.status) && !bars->abort);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (p.splits > 1u) cluster_wait();   // every CTA of the cluster has started
         if (ok) {

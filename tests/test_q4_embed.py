@@ -126,6 +126,11 @@ def test_rows_beyond_four_gigabytes(ops):
     point = torch.tensor(list(mx.VALUES), dtype=torch.bfloat16, device="cuda")
     c = codes[ids]
     assert torch.equal(got, point[torch.stack([c & 15, c >> 4], dim=-1).long()].view(5, n * 32))
+    many = torch.full((20000,), 3, device="cuda")         # 20000 rows of 262144 bytes out: 5.2 GB
+    many[-1], many[16384] = 69999, 65536
+    out = ops.mxfp4_embed(codes, scales, many, rows, n, out_dtype=torch.bfloat16)
+    assert torch.equal(out[-1], got[0]) and torch.equal(out[16384], got[1]) and bool((out[16385:19999] == 0).all())
+    del out
     x = torch.zeros(n * 32, device="cuda")
     x[-1] = 1.0                                           # the last column of every row
     y = ops.mxfp4_matvec(codes, scales, x, rows, n)
