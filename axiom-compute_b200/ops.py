@@ -163,8 +163,10 @@ def _float_type(dtype, name: str) -> int:
 
 
 def _count(value, name: str, least: int = 0) -> int:
+    if type(value) is int and least <= value < 0x80000000:
+        return value
     value = operator.index(value)
-    if not least <= value < 1 << 31:
+    if not least <= value < 0x80000000:
         raise ValueError(f"{name} must be in [{least}, 2^31), got {value}")
     return value
 
@@ -203,8 +205,8 @@ def _call(device: int, fn, *args) -> None:
         _raise_for(rc)
 
 
-def _status_ptr(status: Optional[torch.Tensor], device: int):
-    return None if status is None else _ptr(status, torch.int32, "status", 1, device)
+def _status_ptr(status: torch.Tensor, device: int) -> int:
+    return _ptr(status, torch.int32, "status", 1, device)
 
 
 def mxfp4_scale_bytes(rows: int, n_blocks: int) -> int:
@@ -292,7 +294,7 @@ def mxfp4_matvec(codes: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, row
     else:
         yp = _ptr(y, torch.float32, "y", m_tokens * rows, device)
     _call(device, _lib().axc_cuda_mxfp4_matvec, cp, sp, xp, yp, m_tokens, rows, n_blocks, _raw_stream(device),
-          _status_ptr(status, device))
+          None if status is None else _status_ptr(status, device))
     return y
 
 
@@ -312,23 +314,26 @@ def mxfp4_prefill(w_codes: torch.Tensor, w_scales: torch.Tensor, a_codes: torch.
     else:
         cp = _ptr(c, out_dtype, "c", m_tokens * n_rows, device)
     _call(device, _lib().axc_cuda_mxfp4_prefill, wp, wsp, ap, asp, cp, ct, m_tokens, n_rows, n_blocks, _raw_stream(device),
-          _status_ptr(status, device))
+          None if status is None else _status_ptr(status, device))
     return c
 
 
 def _embed(fn, ptrs, device: int, ids, rows: int, n: int, elems: int, scale, out, out_dtype, status):
-    it = _ID_TYPES.get(ids.dtype)
+    it, ot = _ID_TYPES.get(ids.dtype), _FLOAT_TYPES.get(out_dtype)
     if it is None or not ids.is_cuda or not ids.is_contiguous():
         raise ValueError("ids must be a contiguous int32 or int64 CUDA tensor")
+    if ids.get_device() != device:
+        raise ValueError(f"ids is on {ids.device}, the first operand on cuda:{device}")
+    if ot is None:
+        _float_type(out_dtype, "out_dtype")
     n_ids = _count(ids.numel(), "the number of ids")
-    ot = _float_type(out_dtype, "out_dtype")
-    ip = _ptr(ids, ids.dtype, "ids", 0, device)
     if out is None:
         out = torch.empty(*ids.shape, n * elems, dtype=out_dtype, device=ids.device)
         op = out.data_ptr()
     else:
         op = _ptr(out, out_dtype, "out", n_ids * n * elems, device)
-    _call(device, fn, *ptrs, ip, it, n_ids, op, ot, rows, n, scale, _raw_stream(device), _status_ptr(status, device))
+    _call(device, fn, *ptrs, ids.data_ptr(), it, n_ids, op, ot, rows, n, scale, _raw_stream(device),
+          None if status is None else _status_ptr(status, device))
     return out
 
 
