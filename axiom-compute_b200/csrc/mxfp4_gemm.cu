@@ -1,13 +1,17 @@
-// C[m][n] = sum_k A[m][k] W[n][k] for many tokens, A and W in MXFP4: the form of axc_cuda_mxfp4_prefill that is
-// bound by the tensor cores (tcgen05.mma kind::mxf4, block scales, fp32 accumulators in tensor memory).
+// C[m][n] = sum_k A[m][k] W[n][k] for many tokens, A and W in MXFP4: the form of axc_cuda_mxfp4_prefill that reuses what it
+// reads (tcgen05.mma kind::mxf4, block scales, fp32 accumulators in tensor memory).
 //
 // A pair of CTAs (a cluster of two) computes pieces of 256 weight rows (the MMA's M, 128 TMEM lanes in each CTA) x up to
 // 256 tokens (its N, as many TMEM columns) with tcgen05.mma.cta_group::2: each CTA holds its own 128 weight rows and one
 // half of the tokens, so that per SM 32 KB of codes feed 128 x 256 x 256 products.  One CTA alone would have to read 48 KB
-// through the same shared-memory port.  The pairs are persistent and take the
-// pieces in turn, tokens first, so that the pairs at work share the weights through L2.  (Equal contiguous parts for the
-// pairs, cut at 128 tokens, were measured and are not used: 768 x 9472 x 4096 17.9 us either way, 4096 x 28672 x 8192 329 us
-// against 442 us, where every pair reads weights of its own.)
+// through the same shared-memory port.  The pairs are persistent and take the pieces in turn, tokens first, so that the
+// pairs at work share the weights through L2.  (Equal contiguous parts for the pairs, cut at 128 tokens, were measured and
+// are not used: 768 x 9472 x 4096 17.9 us either way, 4096 x 28672 x 8192 329 us against 442 us, where every pair reads
+// weights of its own.)
+//
+// Measured, bf16 output: 4096 x 28672 x 8192 320 us (6.0 PFLOP/s; 380 us where the power limit has lowered the clock), 2048
+// x 18944 x 4096 58 us (5.5 PFLOP/s) with the tensor pipe busy 72 % of the time.  A stage takes 0.33 to 0.38 us where its
+// MMAs take 0.26: its 35 KB arrive from L2 at 10.8 TB/s over all SMs, and issuing it costs the MMA thread about 600 cycles.
 //
 //   warp 0       one thread: TMA loads of this CTA's codes (128-byte swizzle, stages of 256 columns) and bulk copies
 //                of the scale tiles of its rows and of all 256 tokens
@@ -15,7 +19,7 @@
 //                MMAs of 64 columns and the commit that frees the stage in both CTAs; peer: one thread tells the
 //                leader when its stage has landed
 //   warps 2..9   epilogue: 128 of the 256 columns each to registers, tensor memory is free again, then the stores,
-//                while the next tile's MMAs run
+//                while the next piece's MMAs run
 //
 // The accumulators truncate: measured, a chain of K / 64 MMAs loses up to 1.2e-7 * K / 512 of its value when the scales of
 // a row are far apart, and nothing while all partial sums are multiples of one unit below 2^24.
