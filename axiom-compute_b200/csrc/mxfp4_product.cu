@@ -152,7 +152,7 @@ __device__ __forceinline__ void load_x(const MpArgs& p, uint32_t st, uint32_t t,
     const uint32_t k_total = p.n_blocks * 32u, col = st * 256u + lane * 8u;
     if (col < k_total) {     // k_total is a multiple of 32
         const float4* src = reinterpret_cast<const float4*>(p.x + (uint64_t)t * k_total + col);
-        const float4 a = __ldg(src), b = __ldg(src + 1);
+        const float4 a = src[0], b = src[1];
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
 #pragma unroll

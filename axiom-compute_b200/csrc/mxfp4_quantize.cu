@@ -26,12 +26,13 @@ template <>
 struct Eight<float> {
     float v[8];
     __device__ __forceinline__ void load(const float* p) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        const float4* src = reinterpret_cast<const float4*>(p);
+        const float4 a = src[0], b = src[1];
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     }
     __device__ __forceinline__ void load_edge(const float* p, uint32_t count) {
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) v[i] = i < count ? __ldg(p + i) : 0.0f;
+        for (uint32_t i = 0; i < 8u; ++i) v[i] = i < count ? p[i] : 0.0f;
     }
     __device__ __forceinline__ uint32_t top() const {
         uint32_t t = 0;
@@ -47,7 +48,7 @@ struct EightHalves {
     uint32_t w[4];
     template <typename T>
     __device__ __forceinline__ void load(const T* p) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
         w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
     }
     template <typename T>
@@ -55,7 +56,7 @@ struct EightHalves {
         const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i)
-            w[i] = (2u * i < count ? (uint32_t)__ldg(h + 2u * i) : 0u) | (2u * i + 1u < count ? (uint32_t)__ldg(h + 2u * i + 1u) << 16 : 0u);
+            w[i] = (2u * i < count ? (uint32_t)h[2u * i] : 0u) | (2u * i + 1u < count ? (uint32_t)h[2u * i + 1u] << 16 : 0u);
     }
     __device__ __forceinline__ uint32_t top16() const {
         const uint32_t t = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
@@ -91,9 +92,9 @@ __device__ __forceinline__ uint32_t codes_of(const Eight<T>& x, float inv) {
 
 template <typename T, uint32_t SEGS>   // segments of 256 columns that a warp has under way
 __global__ void __launch_bounds__(256)
-mxfp4_quantize_kernel(const T* __restrict__ x, uint64_t row_stride, uint32_t rows, uint32_t cols, uint32_t n_blocks,
-                      uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint32_t n_groups, uint64_t n_items, int wide) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // an ordered launch: see axc_tuning.pdl
+mxfp4_quantize_kernel(const T* x, uint64_t row_stride, uint32_t rows, uint32_t cols, uint32_t n_blocks,
+                      uint8_t* codes, uint8_t* scales, uint32_t n_groups, uint64_t n_items, int wide) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // an ordered launch: see axc_tuning.pdl.  x may be new: no __ldg, no __restrict__
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t n_quads = (n_blocks + 3u) / 4u;

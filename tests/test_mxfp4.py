@@ -2,6 +2,7 @@
 the format, and their refusals."""
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -340,6 +341,54 @@ def test_matvec_non_finite_x_makes_its_token_nan(ops, value):
     x[1, 100] = value
     y = ops.mxfp4_matvec(dev(codes), dev(tiles), dev(x), 50, 9, m_tokens=3)
     assert bool(torch.isnan(y[1]).all()) and torch.equal(y[0], clean[0]) and torch.equal(y[2], clean[2])
+
+
+@gpu
+def test_matvec_nan_weights_reach_their_row_only(ops):
+    rng = np.random.default_rng(17)
+    codes, scales, _t, _w = mx.random_matrix(300, 9, rng)
+    scales[200, 4] = 255
+    y = ops.mxfp4_matvec(*layout(codes, scales), torch.randn(2, 288, device="cuda"), 300, 9, m_tokens=2).cpu().numpy()
+    want = np.zeros((2, 300), bool)
+    want[:, 200] = True
+    assert np.array_equal(np.isnan(y), want)
+
+
+@gpu
+def test_a_range_of_rows_is_a_matrix(ops):
+    """From a multiple of 128 on, rows can be used by themselves (a shard of a matrix)."""
+    codes, scales, w = large_operands(ops, 500, 20, 5)
+    x = torch.randn(640, device="cuda")
+    whole = ops.mxfp4_matvec(codes, scales, x, 500, 20)
+    part = ops.mxfp4_matvec(codes[256:], scales[2 * 5 * 512:], x, 244, 20)
+    assert bool(((part - whole[256:]).abs() <= chain_bound(20) * 8 * (w.float().abs() @ x.abs())[256:]).all())
+    assert torch.equal(ops.mxfp4_dequant(codes[128:], scales[5 * 512:], 372, 20).double(), w[128:])
+
+
+@gpu
+def test_calls_from_several_threads(ops):
+    codes, scales, w = large_operands(ops, 2000, 64, 6)
+    x = torch.randn(300, 2048, device="cuda")
+    a_codes, a_scales = ops.mxfp4_quantize(x)
+    want = (ops.mxfp4_matvec(codes, scales, x[:4], 2000, 64, m_tokens=4),
+            ops.mxfp4_prefill(codes, scales, a_codes, a_scales, 300, 2000, 64),
+            ops.mxfp4_prefill(codes, scales, a_codes, a_scales, 30, 2000, 64))
+    torch.cuda.synchronize()
+
+    def work(_):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            good = True
+            for _i in range(20):
+                c, s = ops.mxfp4_quantize(x)
+                got = (ops.mxfp4_matvec(codes, scales, x[:4], 2000, 64, m_tokens=4),
+                       ops.mxfp4_prefill(codes, scales, c, s, 300, 2000, 64),
+                       ops.mxfp4_prefill(codes, scales, c, s, 30, 2000, 64))
+                torch.cuda.current_stream().synchronize()
+                good = good and all(torch.equal(g, e) for g, e in zip(got, want))
+            return good
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(4)))
 
 
 @gpu
