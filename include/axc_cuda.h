@@ -319,6 +319,8 @@ int axc_cuda_q4k_prefill_form(const void* q, const uint16_t* a_bf16, float* c, u
  *             ((row / 128) * ceil(n_blocks / 4) + block / 4) * 512 + (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4,
  *           the order in which the tensor cores take scales; bytes that belong to no (row, block) are zero
  *           (axc_cuda_mxfp4_quantize writes them; whoever fills the buffer otherwise must too).
+ * The rows from `first` on, a multiple of 128, are a matrix of their own, such as a shard: codes + first * n_blocks * 16
+ * and scales + first * ceil(n_blocks / 4) * 4.
  * The reference has no such format; it stands beside its Q4_K_M and Q4_0 (examples/q4km_dequant_matvec.axc,
  * examples/q4_0_dequant_matvec.axc). */
 size_t axc_cuda_mxfp4_scale_bytes(uint32_t rows, uint32_t n_blocks);

@@ -366,6 +366,32 @@ def test_a_range_of_rows_is_a_matrix(ops):
 
 
 @gpu
+def test_sizes_beyond_four_gigabytes(ops):
+    """x, codes and the product pass 2^32 bytes, x and the product 2^32 elements too."""
+    rows, nb, m = 1_060_000, 256, 4100
+    ends = torch.cat([torch.arange(300), torch.arange(rows - 300, rows)]).cuda()
+    x = torch.zeros(rows, nb * 32, dtype=torch.bfloat16, device="cuda")
+    x[ends] = torch.randn(600, nb * 32, device="cuda").to(torch.bfloat16)
+    codes, scales = ops.mxfp4_quantize(x)
+    few = ops.mxfp4_quantize(x[ends])
+    del x
+    w = ops.mxfp4_dequant(*few, 600, nb)
+    assert torch.equal(codes[ends], few[0])
+    assert torch.equal(ops.mxfp4_embed(codes, scales, ends, rows, nb), w)
+    a_codes, a_scales = ops.mxfp4_quantize(torch.randn(m, nb * 32, device="cuda"))
+    a = ops.mxfp4_dequant(a_codes, a_scales, m, nb)[-300:].double()
+    half = torch.finfo(torch.bfloat16).eps / 2
+    for tokens in (m, 100):                               # many and few tokens
+        operand = (a_codes, a_scales) if tokens == m else ops.mxfp4_quantize(a[-tokens:].float())
+        c = ops.mxfp4_prefill(codes, scales, *operand, tokens, rows, nb, out_dtype=torch.bfloat16)
+        last = min(tokens, 300)
+        ref, mag = a[-last:] @ w.double().t(), a[-last:].abs() @ w.double().abs().t()
+        assert bool(((c[-last:, ends].double() - ref).abs() <= chain_bound(nb) * mag * (1 + half) + half * ref.abs()).all())
+        assert bool((c[-last:, 300:rows - 300] == 0).all())
+        del c
+
+
+@gpu
 def test_calls_from_several_threads(ops):
     codes, scales, w = large_operands(ops, 2000, 64, 6)
     x = torch.randn(300, 2048, device="cuda")
