@@ -490,15 +490,15 @@ cudaError_t launch(const CUtensorMap& tm_w, const CUtensorMap& tm_a, MpArgs p, c
     return cudaLaunchKernelEx(&cfg, kern, tm_w, tm_a, p);
 }
 
-// CTAs per cluster: K is split as long as each CTA keeps four stages (1024 columns) and all clusters run at once.  A second
-// round of CTAs costs as much as the first (14336 x 4096, one token: 112 CTAs 7.6 us, 224 CTAs 11.5 us), and clusters of 4
-// and 8 do not reach every SM (15 clusters of 8 on 148 SMs; 2000 x 16000, three tokens: 64 CTAs in clusters of 8 7.8 us, 128
-// CTAs 12.6 us).
-uint32_t choose_splits(uint32_t groups, uint32_t n_blocks, uint32_t sms) {
+// CTAs per cluster: K of at least `first` stages of 256 columns is split in two, again and again, as long as all clusters
+// run at once and each half of a share has least / 2 stages.  A second round of CTAs costs as much as the first (14336 x 4096, one token: 112 CTAs 7.5 us, 224
+// CTAs 10.8 us), and clusters of 4 and 8 do not reach every SM (15 clusters of 8 on 148 SMs; 4096 x 14336, one token: 64
+// CTAs in clusters of 8 9.4 us, 128 CTAs 12.5 us).
+uint32_t choose_splits(uint32_t groups, uint32_t n_blocks, uint32_t sms, uint32_t first, uint32_t least) {
     const uint32_t st = (n_blocks + 7u) / 8u;
-    const uint64_t most[4] = {sms, sms, sms * 7u / 8u, sms * 3u / 4u};   // CTAs that run at once in clusters of 1, 2, 4, 8
+    const uint64_t most[4] = {sms, sms, sms * 7u / 8u, sms * 13u / 16u};   // CTAs that run at once in clusters of 1, 2, 4, 8
     uint32_t shift = 0;
-    while (shift < 3u && ((uint64_t)groups << (shift + 1u)) <= most[shift + 1u] && st >= 8u << shift) ++shift;
+    while (shift < 3u && st >= first && ((uint64_t)groups << (shift + 1u)) <= most[shift + 1u] && st >= least << shift) ++shift;
     return 1u << shift;
 }
 
@@ -513,16 +513,22 @@ cudaError_t launch_mxfp4_matvec(const uint8_t* codes, const uint8_t* scales, con
     p.n = (m_tokens + 1u) / 2u * 16u;
     CUtensorMap tm_w;
     if (!mx_encode_codes(&tm_w, codes, rows, n_blocks, MP_ROWS)) return cudaErrorInvalidValue;
-    // Two tiles per CTA halve the work of splitting x, which every CTA does for its share of K (one token, 8192 x 8192: 8.3
-    // us, one tile 9.4 us; 57344 x 8192: 43 us, 50 us).  Rows of three stages or less are too short for it: 40000 x 512
-    // 6.7 us, one tile 5.7 us.
-    const uint32_t row_tiles = (rows + MP_ROWS - 1u) / MP_ROWS;
-    if (row_tiles >= 8u && n_blocks > 24u) {
-        p.splits = choose_splits((row_tiles + 1u) / 2u, n_blocks, (uint32_t)sm_count);
-        return launch<true, 2, float>(tm_w, tm_w, p, stream);
-    }
-    p.splits = choose_splits(row_tiles, n_blocks, (uint32_t)sm_count);
-    return launch<true, 1, float>(tm_w, tm_w, p, stream);
+    // Two tiles per CTA halve the work of splitting x, which every CTA does for its share of K (8192 x 8192, 8 tokens: 11.2
+    // us, one tile 17.2 us), and allow twice the splits (2048 x 8192, one token: 4.6 us, one tile 5.4 us).  A CTA of one
+    // tile starts and ends sooner and needs less per stage.  So one tile where that allows as many splits and either the
+    // share of K is short (one token, 4096 x 2048: 3.2 us, two tiles 3.5 us) or, with few tokens, there are not many CTAs
+    // (2048 x 4096: 3.5 us, two tiles 3.9 us; but 4096 x 4096 4.4 us, two tiles 4.1 us) or much to read for each
+    // (4096 x 14336: 8.5 us, two tiles 9.4 us).  More rows than SMs take two, but for few tokens and the shortest rows
+    // (40000 x 256: 5.1 us, two tiles 5.7 us; 40000 x 2048: 15.2 us, 13.2 us).  The splits do not depend on the number of
+    // tokens, so that a token's sums do not.
+    const uint32_t sms = (uint32_t)sm_count, row_tiles = (rows + MP_ROWS - 1u) / MP_ROWS, st = (n_blocks + 7u) / 8u;
+    const uint32_t one = choose_splits(row_tiles, n_blocks, sms, 4u, 3u), two = choose_splits((row_tiles + 1u) / 2u, n_blocks, sms, 6u, 6u);
+    p.splits = one > two ? one : two;
+    const uint32_t share = (st + p.splits - 1u) / p.splits;
+    const bool few = m_tokens <= 4u;
+    const bool one_tile = one >= two && row_tiles <= sms && (share <= 2u || (few && (share >= 8u || row_tiles * p.splits * 2u <= sms)));
+    if (one_tile || (st <= 3u && few)) return launch<true, 1, float>(tm_w, tm_w, p, stream);
+    return launch<true, 2, float>(tm_w, tm_w, p, stream);
 }
 
 cudaError_t launch_mxfp4_prefill(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* a_codes,
@@ -544,7 +550,7 @@ cudaError_t launch_mxfp4_prefill(const uint8_t* w_codes, const uint8_t* w_scales
     // Two tiles per CTA where one each would need a second round of CTAs: 28672 x 3200, 64 tokens 15.9 -> 12.1 us.
     const uint32_t row_tiles = (n_rows + MP_ROWS - 1u) / MP_ROWS;
     const bool two = row_tiles > (uint32_t)sm_count && m_tokens <= 64u;
-    p.splits = choose_splits(two ? (row_tiles + 1u) / 2u : row_tiles, n_blocks, (uint32_t)sm_count);
+    p.splits = choose_splits(two ? (row_tiles + 1u) / 2u : row_tiles, n_blocks, (uint32_t)sm_count, 8u, 4u);
     switch (type) {
         case ElemType::F32: return two ? launch<false, 2, float>(tm_w, tm_a, p, stream) : launch<false, 1, float>(tm_w, tm_a, p, stream);
         case ElemType::BF16: return two ? launch<false, 2, __nv_bfloat16>(tm_w, tm_a, p, stream) : launch<false, 1, __nv_bfloat16>(tm_w, tm_a, p, stream);

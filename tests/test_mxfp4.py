@@ -461,6 +461,25 @@ def test_matvec_over_the_forms_of_the_kernel(ops, rows, nb):
 
 
 @gpu
+@pytest.mark.parametrize("rows,nb", [(300, 32), (300, 100), (1024, 128), (2048, 64), (2048, 128), (2048, 256), (3500, 448),
+                                     (4096, 64), (4096, 448), (5120, 64), (18900, 24), (19000, 32), (40000, 24)])
+def test_matvec_where_the_split_of_the_work_changes(ops, rows, nb):
+    """One and two row tiles on either side of the rules that choose them: right, and the same bits for every number of
+    tokens."""
+    codes, scales, w = large_operands(ops, rows, nb, rows + nb)
+    x = torch.randn(8, nb * 32, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda")
+    x64 = x.double()
+    top = x64.abs().view(8, nb, 32).amax(dim=2).repeat_interleave(32, dim=1)
+    fixed, mag = 2.0 ** -22 * (top @ w.abs().t()), x64.abs() @ w.abs().t()
+    st = ops.new_status()
+    all8 = ops.mxfp4_matvec(codes, scales, x, rows, nb, m_tokens=8, status=st)
+    assert bool(((all8.double() - x64 @ w.t()).abs() <= fixed + chain_bound(nb) * (4 * mag + 8 * fixed)).all())
+    for m in (1, 2, 3, 4, 5):
+        assert torch.equal(ops.mxfp4_matvec(codes, scales, x[:m], rows, nb, m_tokens=m, status=st).view(m, rows), all8[:m]), m
+    assert int(st.item()) == 0
+
+
+@gpu
 @pytest.mark.parametrize("m,n,nb", [(40, 1100, 600), (64, 9000, 200), (33, 25000, 16), (64, 20000, 50), (100, 3000, 300), (128, 1000, 900),
                                     (128, 19500, 20), (65, 9600, 40), (129, 4000, 130), (1000, 5000, 100), (2048, 9500, 24),
                                     (3, 60000, 9)])
