@@ -24,7 +24,7 @@
 //                rows to the CTA that finishes them (distributed shared memory), and adds what it got in rank order,
 //                so results do not depend on timing.
 //
-// Measured: matvec of one token 4096 x 4096 3.7 us, 14336 x 4096 6.9 us (4.5 TB/s), 57344 x 8192 43 us (5.8 TB/s), five tokens
+// Measured: matvec of one token 4096 x 4096 3.8 us, 14336 x 4096 6.8 us (4.6 TB/s), 57344 x 8192 43 us (5.8 TB/s), five tokens
 // 8192 x 28672 24.7 us (5.1 TB/s); prefill of 37 tokens 4096 x 14336 8.8 us.  What a launch adds to the time that its bytes
 // take is a chain of latencies of about 3 us: x, its digits, the first stage, the MMAs, the cluster, the store.
 //
