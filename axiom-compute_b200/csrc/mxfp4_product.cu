@@ -11,8 +11,8 @@
 //             product.  y is the sum of its eight columns.  A weight never passes through a register.
 //
 // Both are bound by reading W.  A cluster of `splits` CTAs (1, 2, 4 or 8) owns one or two tiles of 128 weight rows (the
-// MMA's M, one TMEM lane each) and all tokens (its N columns); each CTA takes its share of K, so that small matrices
-// too are spread over the SMs and a CTA has most of its share requested from memory at once.  Stages of 256 columns:
+// MMA's M, one TMEM lane each) and all tokens, or 128 of them (its N columns); each CTA takes its share of K, so that small
+// matrices too are spread over the SMs and a CTA has most of its share requested from memory at once.  Stages of 256 columns:
 //
 //   warp 0       TMA loads of the codes of W (and of A), bulk copies of the scale tiles
 //   warps 1, 2   stages in turn: scales from shared into tensor memory (tcgen05.cp), four MMAs of 64 columns per tile and
@@ -47,7 +47,7 @@
 namespace axc {
 namespace {
 
-constexpr uint32_t MP_ROWS = 128;
+constexpr uint32_t MP_ROWS = 128, MP_TOKENS = 128;   // most that a CTA takes of a tile of rows, of tokens
 constexpr uint32_t MP_STAGE_BYTES = 128;            // one stage: 256 columns = 128 bytes of codes per row
 constexpr uint32_t MP_W_BYTES = MP_ROWS * MP_STAGE_BYTES;
 constexpr uint32_t MP_MAX_STAGES = 8;
@@ -216,6 +216,7 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     const uint32_t n_quads = (p.n_blocks + 3u) / 4u, all_st = (p.n_blocks + 7u) / 8u;
     const uint32_t st0 = (uint32_t)((uint64_t)all_st * rank / p.splits);
     const uint32_t n_st = (uint32_t)((uint64_t)all_st * (rank + 1u) / p.splits) - st0;   // at least one
+    const uint32_t tok0 = DIGITS ? 0u : blockIdx.y * MP_TOKENS, m = min(p.m - tok0, MP_TOKENS);   // this CTA's tokens
     const uint32_t b_stage = p.n * MP_STAGE_BYTES;
     const uint32_t w_tiles = min(TILES, (p.rows + 127u) / 128u - tile0);                 // tiles that exist
 
@@ -265,8 +266,9 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
                              p.w_scales + ((uint64_t)(tile0 + i) * n_quads + st * 2u) * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
                 }
                 if (!DIGITS) {
-                    tma_load_2d(base + p.off_b + s * b_stage, &tm_a, (int32_t)(st * MP_STAGE_BYTES), 0, &bars->full[s]);
-                    bulk_g2s(sm + p.off_sfb + s * SFB_STAGE, p.a_scales + (uint64_t)st * 2u * MX_TILE_BYTES, quad_bytes, &bars->full[s]);
+                    tma_load_2d(base + p.off_b + s * b_stage, &tm_a, (int32_t)(st * MP_STAGE_BYTES), (int32_t)tok0, &bars->full[s]);
+                    bulk_g2s(sm + p.off_sfb + s * SFB_STAGE, p.a_scales + ((uint64_t)(tok0 / 128u) * n_quads + st * 2u) * MX_TILE_BYTES,
+                             quad_bytes, &bars->full[s]);
                 }
             }
             __syncwarp();
@@ -357,9 +359,9 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
             if (p.splits > 1u) {
                 asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(base + p.off_red), "r"(lr >> p.per_shift));
                 const uint32_t slot = (rank << p.per_shift) | (lr & ((1u << p.per_shift) - 1u));   // [source][row]
-                dst += slot * red_row<DIGITS>(p.m) * 4u;
+                dst += slot * red_row<DIGITS>(m) * 4u;
             }
-            const uint32_t columns = DIGITS ? p.m * 8u : p.m;
+            const uint32_t columns = DIGITS ? m * 8u : m;
             for (uint32_t c = grp * 8u; c < columns; c += 16u) {
                 uint32_t r0[8], r1[8];
                 tmem_load8(taddr + c, r0);
@@ -381,7 +383,7 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
                                      "f"(sum[j + 1]), "f"(sum[j + 2]), "f"(sum[j + 3])
                                      : "memory");
                 } else if (row < p.rows) {
-                    Out* out = reinterpret_cast<Out*>(p.out) + (uint64_t)c * p.rows + row;
+                    Out* out = reinterpret_cast<Out*>(p.out) + (uint64_t)(tok0 + c) * p.rows + row;
 #pragma unroll
                     for (uint32_t j = 0; j < 8u; ++j)
                         if (c + j < columns) put(out + (uint64_t)j * p.rows, sum[j]);
@@ -395,11 +397,11 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         if (warp < MP_FIRST_X) cluster_wait();
         cluster_sync_all();
         if (warp >= MP_FIRST_X) {
-            const uint32_t per = 1u << p.per_shift, pitch = red_row<DIGITS>(p.m);
+            const uint32_t per = 1u << p.per_shift, pitch = red_row<DIGITS>(m);
             const float* red = reinterpret_cast<const float*>(sm + p.off_red);
             const uint64_t first = (uint64_t)tile0 * MP_ROWS + rank * per;
             constexpr uint32_t WIDE = DIGITS ? 1u : 4u;            // neighbouring columns that a thread adds
-            for (uint32_t i = tid - MP_FIRST_X * 32u; i < (p.m + WIDE - 1u) / WIDE << p.per_shift; i += X_WARPS * 32u) {
+            for (uint32_t i = tid - MP_FIRST_X * 32u; i < (m + WIDE - 1u) / WIDE << p.per_shift; i += X_WARPS * 32u) {
                 const uint32_t r = i & (per - 1u), c = (i >> p.per_shift) * WIDE;
                 float sum[WIDE] = {};
                 for (uint32_t k = 0; k < p.splits; ++k) {
@@ -412,10 +414,10 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
                     }
                 }
                 if (first + r < p.rows) {
-                    Out* out = reinterpret_cast<Out*>(p.out) + (uint64_t)c * p.rows + first + r;
+                    Out* out = reinterpret_cast<Out*>(p.out) + (uint64_t)(tok0 + c) * p.rows + first + r;
 #pragma unroll
                     for (uint32_t j = 0; j < WIDE; ++j)
-                        if (c + j < p.m) put(out + (uint64_t)j * p.rows, sum[j]);
+                        if (c + j < m) put(out + (uint64_t)j * p.rows, sum[j]);
                 }
             }
         }
@@ -437,7 +439,7 @@ cudaError_t launch(const CUtensorMap& tm_w, const CUtensorMap& tm_a, MpArgs p, c
     // shared memory: W stages, B stages, scales of W and B, what the cluster sends, barriers
     const uint32_t w_stage = TILES * MP_W_BYTES, b_stage = p.n * MP_STAGE_BYTES, sfw_stage = TILES * 1024u;
     const uint32_t per_stage = w_stage + b_stage + sfw_stage + 1024u;
-    const uint32_t red = p.splits > 1u ? TILES * MP_ROWS * red_row<DIGITS>(p.m) * 4u : 0u;
+    const uint32_t red = p.splits > 1u ? TILES * MP_ROWS * red_row<DIGITS>(p.m < MP_TOKENS ? p.m : MP_TOKENS) * 4u : 0u;
     const uint32_t fixed = 1024u + (uint32_t)sizeof(MpBars) + red;
     uint32_t stages = (MP_SMEM_MAX - fixed) / per_stage;
     if (stages > MP_MAX_STAGES) stages = MP_MAX_STAGES;
@@ -478,7 +480,7 @@ cudaError_t launch(const CUtensorMap& tm_w, const CUtensorMap& tm_a, MpArgs p, c
     }
     const uint32_t row_tiles = (p.rows + MP_ROWS - 1u) / MP_ROWS;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((row_tiles + TILES - 1u) / TILES * p.splits);
+    cfg.gridDim = dim3((row_tiles + TILES - 1u) / TILES * p.splits, (p.m + MP_TOKENS - 1u) / MP_TOKENS);
     cfg.blockDim = dim3(mp_threads(TILES));
     cfg.dynamicSmemBytes = smem, cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -536,21 +538,26 @@ cudaError_t launch_mxfp4_prefill(const uint8_t* w_codes, const uint8_t* w_scales
                                  uint32_t n_blocks, uint32_t* status, cudaStream_t stream, int sm_count) {
     if (m_tokens == 0 || n_rows == 0 || n_blocks == 0) return cudaSuccess;
     if (!tensor_map_encoder()) return cudaErrorNotSupported;
-    // Beyond 64 tokens the form for many tokens where its pairs of CTAs have a row tile each (128 tokens, 28672 x 8192: 29.8
-    // us, this form 33.8 us), beyond 128 always; this form splits K (128 tokens, 4096 x 14336: 12.5 us, the other 20.7 us).
-    if (m_tokens > 128u || (m_tokens > 64u && (uint64_t)n_rows >= 128ull * (uint64_t)sm_count))
+    // Which form: this one splits K, the one for many tokens reads W and A less often.  Up to 128 tokens this one, beyond 64
+    // unless the other has a row tile for each of its pairs of CTAs (128 tokens, 28672 x 8192: 29.8 us, this form 33.8 us;
+    // 4096 x 14336: 20.7 us, this form 12.5 us).  Beyond 128 this one where rows and tokens leave SMs to split long rows over
+    // (256 tokens, 4096 x 14336: 15.7 us, the other 20.7 us, 1024 x 14336: 10.4 us, 20.3 us; but 4096 x 1024: 5.7 us, 5.6 us, and
+    // without a split 1024 tokens, 4096 x 14336: 40.8 us, 20.9 us).
+    const uint32_t sms = (uint32_t)sm_count, row_tiles = (n_rows + MP_ROWS - 1u) / MP_ROWS;
+    const uint32_t chunks = (m_tokens + MP_TOKENS - 1u) / MP_TOKENS;
+    // Two tiles per CTA where one each would need a second round of CTAs: 28672 x 3200, 64 tokens 15.9 -> 12.1 us.
+    const bool two = row_tiles > sms && m_tokens <= 64u;
+    const uint64_t groups = (uint64_t)(two ? (row_tiles + 1u) / 2u : row_tiles) * chunks;
+    const uint32_t splits = groups > sms ? 1u : choose_splits((uint32_t)groups, n_blocks, sms, 8u, 4u);
+    if (chunks > 1u ? splits == 1u || n_blocks < 128u : m_tokens > 64u && row_tiles >= sms)
         return launch_mxfp4_gemm(w_codes, w_scales, a_codes, a_scales, c, type, m_tokens, n_rows, n_blocks, status, stream, sm_count);
     MpArgs p{};
     p.w_scales = w_scales, p.a_scales = a_scales, p.out = c, p.m = m_tokens, p.rows = n_rows, p.n_blocks = n_blocks;
-    p.status = status;
-    p.n = (m_tokens + 15u) / 16u * 16u;
+    p.status = status, p.splits = splits;
+    p.n = chunks > 1u ? MP_TOKENS : (m_tokens + 15u) / 16u * 16u;
     CUtensorMap tm_w, tm_a;
     if (!mx_encode_codes(&tm_w, w_codes, n_rows, n_blocks, MP_ROWS) || !mx_encode_codes(&tm_a, a_codes, m_tokens, n_blocks, p.n))
         return cudaErrorInvalidValue;
-    // Two tiles per CTA where one each would need a second round of CTAs: 28672 x 3200, 64 tokens 15.9 -> 12.1 us.
-    const uint32_t row_tiles = (n_rows + MP_ROWS - 1u) / MP_ROWS;
-    const bool two = row_tiles > (uint32_t)sm_count && m_tokens <= 64u;
-    p.splits = choose_splits(two ? (row_tiles + 1u) / 2u : row_tiles, n_blocks, (uint32_t)sm_count, 8u, 4u);
     switch (type) {
         case ElemType::F32: return two ? launch<false, 2, float>(tm_w, tm_a, p, stream) : launch<false, 1, float>(tm_w, tm_a, p, stream);
         case ElemType::BF16: return two ? launch<false, 2, __nv_bfloat16>(tm_w, tm_a, p, stream) : launch<false, 1, __nv_bfloat16>(tm_w, tm_a, p, stream);

@@ -480,6 +480,23 @@ def test_matvec_where_the_split_of_the_work_changes(ops, rows, nb):
 
 
 @gpu
+@pytest.mark.parametrize("m,n,nb", [(129, 4096, 128), (160, 300, 130), (200, 1000, 448), (257, 2100, 256), (300, 4500, 127), (513, 260, 130),
+                                    (640, 900, 200), (1000, 129, 300), (2000, 128, 128), (4096, 100, 140), (130, 9400, 128), (130, 9500, 128)])
+def test_prefill_of_rows_split_over_the_sms(ops, m, n, nb):
+    """More than 128 tokens and few rows: on either side of the rule that splits K, and nothing beyond the output."""
+    w_codes, w_scales, w = large_operands(ops, n, nb, n + nb)
+    a_codes, a_scales, a = large_operands(ops, m, nb, m + nb, 3.0)
+    st = ops.new_status()
+    out = torch.full((m * n + 300,), 7.0, device="cuda")
+    ops.mxfp4_prefill(w_codes, w_scales, a_codes, a_scales, m, n, nb, c=out, status=st)
+    c = out[:m * n].view(m, n)
+    assert int(st.item()) == 0 and bool((out[m * n:] == 7.0).all())
+    assert bool(((c.double() - a @ w.t()).abs() <= chain_bound(nb) * (a.abs() @ w.abs().t())).all())
+    for dtype in (torch.bfloat16, torch.float16):         # the same sums, rounded once
+        assert torch.equal(ops.mxfp4_prefill(w_codes, w_scales, a_codes, a_scales, m, n, nb, out_dtype=dtype), c.to(dtype))
+
+
+@gpu
 @pytest.mark.parametrize("m,n,nb", [(40, 1100, 600), (64, 9000, 200), (33, 25000, 16), (64, 20000, 50), (100, 3000, 300), (128, 1000, 900),
                                     (128, 19500, 20), (65, 9600, 40), (129, 4000, 130), (1000, 5000, 100), (2048, 9500, 24),
                                     (3, 60000, 9)])
