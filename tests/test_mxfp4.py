@@ -604,3 +604,99 @@ def test_two_streams_at_once(ops):
             got.append(("y", ops.mxfp4_matvec(wd, ws, x, 4096, 128, m_tokens=8)))
     torch.cuda.synchronize()
     assert all(torch.equal(v, c if k == "c" else y) for k, v in got)
+
+
+# ---- the ends of the ranges, with results that are normal numbers ----
+
+
+def pick_columns(rows, blocks, byte):
+    """Codes and scale bytes of a matrix whose row r is 2^(byte - 127) at column r and zero elsewhere."""
+    codes = np.zeros((rows, blocks * 16), np.uint8)
+    r = np.arange(rows)
+    codes[r, r // 2] = 2 << (4 * (r % 2))
+    return codes, np.full((rows, blocks), byte, np.uint8)
+
+
+def held(x):
+    """x as the matvec holds it: per block of 32 columns a whole number of units of 2^(floor(log2 max |x|) - 21), at
+    least 2^-127, ties to even.  The unit is a power of two, so the division is exact in float64."""
+    v = x.astype(np.float64).reshape(x.shape[0], -1, 32)
+    top = np.abs(v).max(axis=2, keepdims=True)
+    _m, e = np.frexp(np.where(top == 0, 1.0, top))
+    unit = np.maximum(np.exp2(np.where(top == 0, -127.0, e - 22.0)), 2.0 ** -127)
+    return (np.rint(v / unit) * unit).reshape(x.shape)
+
+
+@gpu
+@pytest.mark.parametrize("rows,nb,byte", [(128, 4, 147), (128, 5, 254), (300, 64, 150), (2048, 64, 160), (2048, 900, 147)])
+def test_matvec_holds_x_to_its_block_unit(ops, rows, nb, byte):
+    """Each y is one value of x times a power of two, a normal number that the sums hold exactly: tiny and subnormal
+    blocks beside ordinary ones, blocks on either side of 2^-105, and blocks with one value that dwarfs the others."""
+    rng = np.random.default_rng(rows + nb + byte)
+    up = 40 if byte == 254 else 126                       # 2^127 times the largest result stays finite
+    kinds = [(-149, -149), (-149, -126), (-149, -106), (-127, -105), (-106, -104), (-20, 0), (-1, up - 40)]
+    if byte == 254:
+        kinds = kinds[:5] + [(-120, -100), (-60, -20)]
+    x = np.zeros((8, nb, 32))
+    for t in range(8):
+        for b in range(nb):
+            low, high = kinds[(b + t) % len(kinds)]
+            x[t, b] = rng.uniform(-1, 1, 32) * np.exp2(rng.uniform(low, high, 32))
+            x[t, b, rng.integers(32)] = np.exp2(float(high)) * (1.0 if (b + t) % 2 else 0.999)
+    with np.errstate(under="ignore"):
+        x = x.reshape(8, nb * 32).astype(np.float32)
+    codes, tiles = layout(*pick_columns(rows, nb, byte))
+    want = held(x)[:, :rows] * 2.0 ** (byte - 127)
+    assert (np.abs(want[want != 0]) >= 2.0 ** -126).all() and np.abs(want).max() < 2.0 ** 127
+    for m in (1, 3, 8):
+        y = ops.mxfp4_matvec(codes, tiles, dev(x[:m]), rows, nb, m_tokens=m).double().cpu().numpy().reshape(m, rows)
+        assert np.array_equal(y, want[:m]), (m, np.argwhere(y != want[:m])[:5])
+
+
+@gpu
+@pytest.mark.parametrize("power", [-128, -127, -118, -110, -106])
+def test_matvec_of_tiny_x_keeps_the_unit(ops, power):
+    """Sums over whole rows of blocks below 2^-105: the error is half a unit of 2^-127 per column, with a result that an
+    answer of zero would miss (every product is positive)."""
+    rng = np.random.default_rng(21 - power)
+    nb, rows = 6, 200
+    codes, scales, _t, w = mx.random_matrix(rows, nb, rng, 150, 152)
+    codes &= 0x77
+    codes |= 0x22                                         # magnitudes of at least 1
+    w = mx.values(codes, scales)
+    x = (rng.uniform(0.6, 0.99, (2, nb * 32)) * np.exp2(float(power) + 1)).astype(np.float32)
+    y = ops.mxfp4_matvec(*layout(codes, scales), dev(x), rows, nb, m_tokens=2).double().cpu().numpy()
+    x64 = x.astype(np.float64)
+    ref, fixed = x64 @ w.T, 2.0 ** -128 * np.abs(w).sum(axis=1)
+    assert (ref > 1.2 * fixed + chain_bound(nb) * (4 * ref + 8 * fixed)).all()   # so zeros fail
+    assert (np.abs(y - ref) <= fixed + chain_bound(nb) * (4 * ref + 8 * fixed)).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_dequant_and_lookup_overflow_to_infinity(ops, dtype):
+    """Values beyond the output type's range are infinite, not its largest number; every scale byte, every code."""
+    scales = np.arange(256, dtype=np.uint8).reshape(64, 4)
+    codes = np.tile(np.arange(256, dtype=np.uint8), 16).reshape(64, 64)
+    w = ops.mxfp4_dequant(*layout(codes, scales), 64, 4, out_dtype=dtype).cpu()
+    with np.errstate(over="ignore"):
+        ref = torch.from_numpy(mx.values(codes, scales).astype(np.float32)).to(dtype)
+    ok = ~torch.isnan(ref)
+    assert torch.equal(torch.isnan(w), ~ok) and torch.equal(w[ok], ref[ok]) and bool(torch.isinf(ref).any())
+    assert torch.equal(torch.signbit(w[ok]), torch.signbit(ref[ok]))
+    ids = torch.arange(63, -1, -1, device="cuda")
+    e = ops.mxfp4_embed(*layout(codes, scales), ids, 64, 4, out_dtype=dtype).cpu().flip(0)
+    assert torch.equal(torch.isnan(e), ~ok) and torch.equal(e[ok], ref[ok])
+
+
+@gpu
+@pytest.mark.parametrize("m,n,nb", [(5, 130, 3), (40, 300, 40), (300, 600, 5), (200, 300, 130)])
+def test_prefill_overflows_to_infinity(ops, m, n, nb):
+    """Sums beyond fp16 are infinite with the sum's sign, in every form of the product."""
+    rng = np.random.default_rng(m + n)
+    w, a = mx.random_matrix(n, nb, rng, 130, 134), mx.random_matrix(m, nb, rng, 130, 134)
+    args = (dev(w[0]), dev(w[2]), dev(a[0]), dev(a[2]), m, n, nb)
+    c = ops.mxfp4_prefill(*args)
+    half = ops.mxfp4_prefill(*args, out_dtype=torch.float16)
+    assert bool((c.abs() > 65520).any()) and bool((c.abs() < 65504).any())
+    assert torch.equal(half, c.to(torch.float16)) and bool(torch.isinf(half).any())
