@@ -17,11 +17,7 @@ namespace axc {
 
 constexpr int MX_BLOCK = 32;          // values per scale
 constexpr int MX_BLOCK_BYTES = 16;
-constexpr uint32_t MX_TILE_ROWS = 128, MX_TILE_BLOCKS = 4, MX_TILE_BYTES = 512;
-
-__host__ __device__ __forceinline__ uint64_t mx_scale_bytes(uint64_t rows, uint64_t n_blocks) {
-    return (rows + 127u) / 128u * ((n_blocks + 3u) / 4u) * MX_TILE_BYTES;
-}
+constexpr uint32_t MX_TILE_BYTES = 512;   // scales of 128 rows x 4 blocks
 
 // Kernels that stream rows give a warp one segment of 256 columns at a time up to this many segments (two rounds of the
 // warps of all SMs), and four beyond.

@@ -998,6 +998,8 @@ int axc_cuda_mxfp4_dequant(const void* codes, const void* scales, void* w, uint3
     return launch_result(axc::launch_mxfp4_embed((const uint8_t*)codes, (const uint8_t*)scales, nullptr, 0, rows, rows, n_blocks, 1.0f, w, t, nullptr, (cudaStream_t)stream));
 }
 
+static_assert(AXC_MXFP4_MATVEC_TOKENS == axc::MX_MATVEC_TOKENS, "the limit of the header is the kernel's");
+
 int axc_cuda_mxfp4_matvec(const void* codes, const void* scales, const float* x, float* y, uint32_t m_tokens, uint32_t rows,
                           uint32_t n_blocks, void* stream, uint32_t* status) {
     clear_error();

@@ -54,6 +54,7 @@ constexpr uint32_t MP_MAX_STAGES = 8;
 constexpr uint32_t MP_PREFETCH = 16;                // stages requested into L2 before the dependency wait
 constexpr uint32_t MP_MMA_WARPS = 2;
 constexpr uint32_t MP_FIRST_X = 1 + MP_MMA_WARPS;   // the first of the warps that split x and run the epilogue
+static_assert(MX_MATVEC_TOKENS * 8u <= MP_TOKENS / 2u, "eight columns per token: at most 64, see the tensor memory of two tiles");
 // A unit of 256 columns of one token takes such a warp about 1500 cycles, most of them waiting: with two tiles, where a
 // CTA has the SM to itself, 16 of them (8 tokens, 14336 x 4096: 10.7 us, with 8 warps 12.4 us).
 __host__ __device__ constexpr uint32_t mp_x_warps(uint32_t tiles) { return 8u * tiles; }

@@ -112,7 +112,7 @@ struct TableMx {
 // ids: nullptr (row i of the output is row i of the table), or 32-bit / 64-bit numbers.
 template <template <int> class Table, typename Out, uint32_t SEGS>
 __global__ void __launch_bounds__(256)
-rows_kernel(const Table<16 / sizeof(Out)> table, const void* ids, int ids64, uint32_t n_ids, uint32_t rows,
+rows_kernel(const Table<16 / sizeof(Out)> table, const void* ids, int ids64, uint32_t rows,
             float factor, Out* out, uint32_t n_groups, uint64_t n_items, uint32_t* status) {
     constexpr uint32_t V = 16 / sizeof(Out), SEG = 32u * V;
     using T = Table<V>;
@@ -178,7 +178,7 @@ cudaError_t launch_segs(const RowsArgs& a, cudaStream_t stream) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr, cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, rows_kernel<Table, Out, SEGS>, table, a.ids, a.ids64, a.n_ids, a.rows, a.factor,
+    return cudaLaunchKernelEx(&cfg, rows_kernel<Table, Out, SEGS>, table, a.ids, a.ids64, a.rows, a.factor,
                               (Out*)a.out, n_groups, n_items, a.status);
 }
 

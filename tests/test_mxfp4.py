@@ -700,3 +700,12 @@ def test_prefill_overflows_to_infinity(ops, m, n, nb):
     half = ops.mxfp4_prefill(*args, out_dtype=torch.float16)
     assert bool((c.abs() > 65520).any()) and bool((c.abs() < 65504).any())
     assert torch.equal(half, c.to(torch.float16)) and bool(torch.isinf(half).any())
+
+
+def test_the_limit_of_tokens_is_one_number(ffi, ops):
+    """The header's, the binding's and the kernel's limit of the matvec agree (the C entry names the kernel's)."""
+    with open(f"{ROOT}/include/axc_cuda.h") as f:
+        assert f"#define AXC_MXFP4_MATVEC_TOKENS {ops.MX_MATVEC_TOKENS}\n" in f.read()
+    n = ffi.AXC_MXFP4_MATVEC_TOKENS + 1
+    assert ffi.lib().axc_cuda_mxfp4_matvec(16, 32, 48, 64, n, 1, 1, None, None) == ffi.AXC_ERR_INVALID_ARGUMENT
+    assert f"1..{ops.MX_MATVEC_TOKENS} tokens" in ffi.last_error_detail()
