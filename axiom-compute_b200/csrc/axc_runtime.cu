@@ -1039,12 +1039,13 @@ int axc_cuda_mxfp4_prefill(const void* w_codes, const void* w_scales, const void
     return launch_result(e);
 }
 
-static int check_embed(const void* q, const void* scales, const void* ids, uint32_t ids_type, uint32_t n_ids, const void* out,
-                       uint32_t out_type, axc::ElemType* t) {
+// A table without rows (a rank of a sharded vocabulary that has none) is never read and may be null.
+static int check_embed(const void* q, const void* scales, const void* ids, uint32_t ids_type, uint32_t n_ids, uint32_t rows,
+                       uint32_t n, const void* out, uint32_t out_type, axc::ElemType* t) {
     if (!elem_type(out_type, t)) return fail(AXC_ERR_INVALID_ARGUMENT, "out must be fp32, bf16 or fp16");
     if (ids_type != AXC_TY_I32 && ids_type != AXC_TY_I64) return fail(AXC_ERR_INVALID_ARGUMENT, "ids must be int32 or int64");
-    if (n_ids == 0) return AXC_OK;
-    int rc = check_dev_ptrs(q, scales, out);
+    if (n_ids == 0 || n == 0) return AXC_OK;
+    int rc = rows == 0 ? check_dev_ptrs(out, out, out) : check_dev_ptrs(q, scales, out);
     if (rc != AXC_OK) return rc;
     if (!ids || (uintptr_t)ids % (ids_type == AXC_TY_I64 ? 8 : 4))
         return fail(AXC_ERR_INVALID_ARGUMENT, "ids must be non-null and aligned to their type");
@@ -1055,7 +1056,7 @@ int axc_cuda_q4k_embed(const void* q, const void* ids, uint32_t ids_type, uint32
                        uint32_t rows, uint32_t n_superblocks, float scale, void* stream, uint32_t* status) {
     clear_error();
     axc::ElemType t = axc::ElemType::F32;
-    int rc = n_superblocks == 0 ? check_embed(ids, ids, ids, ids_type, 0, out, out_type, &t) : check_embed(q, q, ids, ids_type, n_ids, out, out_type, &t);
+    int rc = check_embed(q, q, ids, ids_type, n_ids, rows, n_superblocks, out, out_type, &t);
     if (rc != AXC_OK) return rc;
     if (n_superblocks >= (1u << 23)) return fail(AXC_ERR_INVALID_ARGUMENT, "embed shape out of range");
     return launch_result(axc::launch_q4k_embed((const uint8_t*)q, ids, ids_type == AXC_TY_I64, n_ids, rows, n_superblocks, scale, out, t, status, (cudaStream_t)stream));
@@ -1065,7 +1066,7 @@ int axc_cuda_q4_0_embed(const void* q, const void* ids, uint32_t ids_type, uint3
                         uint32_t rows, uint32_t n_blocks, float scale, void* stream, uint32_t* status) {
     clear_error();
     axc::ElemType t = axc::ElemType::F32;
-    int rc = n_blocks == 0 ? check_embed(ids, ids, ids, ids_type, 0, out, out_type, &t) : check_embed(q, q, ids, ids_type, n_ids, out, out_type, &t);
+    int rc = check_embed(q, q, ids, ids_type, n_ids, rows, n_blocks, out, out_type, &t);
     if (rc != AXC_OK) return rc;
     if (n_blocks >= (1u << 26)) return fail(AXC_ERR_INVALID_ARGUMENT, "embed shape out of range");
     return launch_result(axc::launch_q4_0_embed((const uint8_t*)q, ids, ids_type == AXC_TY_I64, n_ids, rows, n_blocks, scale, out, t, status, (cudaStream_t)stream));
@@ -1075,7 +1076,7 @@ int axc_cuda_mxfp4_embed(const void* codes, const void* scales, const void* ids,
                          uint32_t out_type, uint32_t rows, uint32_t n_blocks, float scale, void* stream, uint32_t* status) {
     clear_error();
     axc::ElemType t = axc::ElemType::F32;
-    int rc = n_blocks == 0 ? check_embed(ids, ids, ids, ids_type, 0, out, out_type, &t) : check_embed(codes, scales, ids, ids_type, n_ids, out, out_type, &t);
+    int rc = check_embed(codes, scales, ids, ids_type, n_ids, rows, n_blocks, out, out_type, &t);
     if (rc != AXC_OK) return rc;
     if (n_blocks >= (1u << 26)) return fail(AXC_ERR_INVALID_ARGUMENT, "embed shape out of range");
     return launch_result(axc::launch_mxfp4_embed((const uint8_t*)codes, (const uint8_t*)scales, ids, ids_type == AXC_TY_I64, n_ids, rows, n_blocks, scale, out, t, status, (cudaStream_t)stream));

@@ -356,7 +356,8 @@ int axc_cuda_mxfp4_prefill(const void* w_codes, const void* w_scales, const void
  * out[i] = round(dequant(row ids[i]) * scale): the fp32 values of the *_dequant calls, multiplied in fp32, rounded
  * once to out_type.  ids: n_ids numbers of ids_type AXC_TY_I32 or AXC_TY_I64 in device memory, any order, repeats
  * allowed.  An id outside [0, rows) (say -1 for padding) reads nothing: its row of out is zero and bit 1 (value 2)
- * of *status (nullable) is set.  out: n_ids rows, 16-byte aligned. */
+ * of *status (nullable) is set; with rows = 0 that is every id, and the table may be null.  out: n_ids rows, 16-byte
+ * aligned. */
 int axc_cuda_q4k_embed(const void* q, const void* ids, uint32_t ids_type, uint32_t n_ids, void* out, uint32_t out_type,
                        uint32_t rows, uint32_t n_superblocks, float scale, void* stream, uint32_t* status);
 int axc_cuda_q4_0_embed(const void* q, const void* ids, uint32_t ids_type, uint32_t n_ids, void* out, uint32_t out_type,

@@ -167,3 +167,19 @@ def test_tied_table_from_embedding_to_head(ops, synth):
     ids.copy_(torch.randint(0, rows, (33,), device="cuda"))
     graph.replay()
     check(*out)
+
+
+@gpu
+@pytest.mark.parametrize("fmt,blocks", [("q4k", 2), ("q4_0", 3), ("mxfp4", 5)])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+def test_a_table_without_rows_gives_zero_rows(ops, fmt, blocks, out_dtype):
+    """Every id is outside it: zeros and the status bit, and nothing is read."""
+    e = torch.empty(0, dtype=torch.uint8, device="cuda")
+    args = (e, e) if fmt == "mxfp4" else (e,)
+    st = ops.new_status()
+    cols = blocks * (256 if fmt == "q4k" else 32)
+    out = torch.full((3, cols), 9.0, dtype=out_dtype, device="cuda")
+    ids = torch.tensor([0, -1, 7], device="cuda")
+    getattr(ops, fmt + "_embed")(*args, ids, 0, blocks, out=out, out_dtype=out_dtype, status=st)
+    assert bool((out == 0).all()) and int(st.item()) == 2
+    assert getattr(ops, fmt + "_embed")(*args, ids[:0], 0, blocks).shape == (0, cols)
