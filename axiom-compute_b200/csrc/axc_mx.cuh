@@ -20,7 +20,7 @@ constexpr int MX_BLOCK_BYTES = 16;
 constexpr uint32_t MX_TILE_BYTES = 512;   // scales of 128 rows x 4 blocks
 
 // Kernels that stream rows give a warp one segment of 256 columns at a time up to this many segments (two rounds of the
-// warps of all SMs), and four beyond.
+// 64 warps of each of a B200's 148 SMs), and four beyond.
 constexpr uint64_t SMALL_SEGMENTS = 148u * 64u * 2u;
 
 // Byte offset of the scales of blocks 4 * quad .. 4 * quad + 3 of a row; n_quads = ceil(n_blocks / 4).

@@ -9,9 +9,10 @@
 // are not used: 768 x 9472 x 4096 17.9 us either way, 4096 x 28672 x 8192 329 us against 442 us, where every pair reads
 // weights of its own.)
 //
-// Measured, bf16 output: 4096 x 28672 x 8192 320 us (6.0 PFLOP/s; 380 us where the power limit has lowered the clock), 2048
-// x 18944 x 4096 58 us (5.5 PFLOP/s) with the tensor pipe busy 72 % of the time.  A stage takes 0.33 to 0.38 us where its
-// MMAs take 0.26: its 35 KB arrive from L2 at 10.8 TB/s over all SMs, and issuing it costs the MMA thread about 600 cycles.
+// Measured, bf16 output: 4096 x 28672 x 8192 320 us (6.0 PFLOP/s; 377 us where the power limit has lowered the clock), 2048
+// x 18944 x 4096 58 us (5.5 PFLOP/s; 67 us sustained) with the tensor pipe busy 72 % of the time.  At 0.26 us of MMAs per
+// stage of a pair the first would take 201 us: the rest are stages that wait.  A stage takes 0.33 to 0.38 us where its MMAs
+// take 0.26: its 35 KB arrive from L2 at 10.8 TB/s over all SMs, and issuing it costs the MMA thread about 600 cycles.
 //
 //   warp 0       one thread: TMA loads of this CTA's codes (128-byte swizzle, stages of 256 columns) and bulk copies
 //                of the scale tiles of its rows and of all 256 tokens
@@ -21,8 +22,11 @@
 //   warps 2..9   epilogue: 128 of the 256 columns each to registers, tensor memory is free again, then the stores,
 //                while the next piece's MMAs run
 //
-// The accumulators truncate: measured, a chain of K / 64 MMAs loses up to 1.2e-7 * K / 512 of its value when the scales of
-// a row are far apart, and nothing while all partial sums are multiples of one unit below 2^24.
+// The accumulators truncate: each of the K / 64 MMAs of a chain cuts off at most 2^-22 of the running sum, and nothing while
+// all partial sums are multiples of one unit below 2^24.  Measured on positive products with scales 24 binades apart, where
+// it is worst: 2.0e-10 to 2.4e-10 of the value per column on average, always towards zero, and at most 7.0e-6 at K = 14336;
+// with products of both signs 5.2e-6 of sum |A W|.  Shorter chains, emptied on the way and added in fp32, would lose less at
+// the cost of an epilogue's loads for every part; they are not built.
 //
 // Every wait on an mbarrier is bounded; a wait that runs out sets an error bit and an abort flag, all roles fall
 // through to the common exit, outstanding copies are waited for and tensor memory is freed.

@@ -3,9 +3,12 @@
 //
 //   prefill   C[m][n] = sum_k A[m][k] W[n][k], A in MXFP4 too: the operands go from memory to the tensor cores as
 //             they lie there, codes through TMA (128-byte swizzle), scales through shared into tensor memory.
-//   matvec    y[t][r] = sum_k W[r][k] x[t][k] for a few fp32 vectors x, without rounding them to 4 bits: within each
-//             block of 32 columns x is a 23-bit integer X times a power of two, and X is written in eight digits of
-//             base 8, v_0 .. v_7 in -4 .. 3, X = sum v_d 8^d.  Every digit is an E2M1 value (half of it is one of
+//   matvec    y[t][r] = sum_k W[r][k] x[t][k] for a few fp32 vectors x.  They are rounded, though not to 4 bits: within
+//             each block of 32 columns x is a 23-bit integer X with sign times a power of two, off by at most 2^-22 of
+//             the block's largest |x| (an fp32 is off by 2^-24 of each value: a value beside one 2^20 times as large
+//             keeps two bits).  X is written in eight digits of base 8, v_0 .. v_7 in -4 .. 3, X = sum v_d 8^d, which
+//             is what one step of eight columns holds; more digits would widen every MMA and double the work of
+//             splitting x.  Every digit is an E2M1 value (half of it is one of
 //             0, 0.5, 1, 1.5, 2, whose codes count 0, 1, 2, 3, 4), so one token is eight rows of an MXFP4 matrix
 //             that differ in their scales by factors of 8, and the product with these rows is the same tensor-core
 //             product.  y is the sum of its eight columns.  A weight never passes through a register.
@@ -24,18 +27,23 @@
 //                rows to the CTA that finishes them (distributed shared memory), and adds what it got in rank order,
 //                so results do not depend on timing.
 //
-// Measured: matvec of one token 4096 x 4096 3.8 us, 14336 x 4096 6.8 us (4.6 TB/s), 57344 x 8192 43 us (5.8 TB/s), five tokens
-// 8192 x 28672 24.7 us (5.1 TB/s); prefill of 37 tokens 4096 x 14336 8.8 us.  What a launch adds to the time that its bytes
-// take is a chain of latencies of about 3 us: x, its digits, the first stage, the MMAs, the cluster, the store.
+// Measured, ordered launches back to back, weights that rotate over more than 640 MB (in brackets: the same weights again,
+// which up to 126 MB lie in L2): matvec of one token 4096 x 4096 4.1 us (3.8), 14336 x 4096 7.4 us (6.6), 57344 x 8192 43.7 us
+// (5.7 TB/s); five tokens 8192 x 28672 25.4 us (4.9 TB/s), eight 14336 x 4096 10.5 us; prefill of 37 tokens 4096 x 14336
+// 9.1 us (8.6), of 128 12.4 us (11.5), of 256 15.8 us (15.1).  What an ordered launch adds to the time that its bytes take is
+// a chain of latencies of about 3 us: x, its digits, the first stage, the MMAs, the cluster, the store.  With eight tokens the
+// digits take as long again (every CTA splits x for its share of K), with more than 64 tokens the exchange of partial sums.
 //
 // Each place of the ring has its scale columns in tensor memory, which are free again when the place is.  The
-// accumulators truncate: measured, up to 1.2e-7 of the value per 8 MMAs of a chain when the scales of a row are far apart
-// (and nothing while all partial sums are multiples of one unit below 2^24); a chain is half of a CTA's share of K, and
-// the parts are added in fp32.
+// accumulators truncate: each MMA (64 columns) of a chain cuts off at most 2^-22 of the running sum, and nothing while all
+// partial sums are multiples of one unit below 2^24.  Measured on positive products with scales 24 binades apart, where it
+// is worst: 2.2e-10 of the value per column of a chain on average, always towards zero.  A chain is half of a CTA's share of
+// K, and the parts are added in fp32 (300 x 1024 x 14336, chains of 1792 columns: 4.0e-7 on average, 1.1e-6 at most).
 //
 // Tensor memory and clusters: a CTA that waits for its cluster while another of the cluster waits for tensor memory
 // could wait for good, so a CTA's shared memory is at least its share of tensor memory (columns / 512 of an SM), and
-// whatever fits an SM finds its columns.
+// whatever fits an SM finds its columns.  (They may lie anywhere: by their registers no more than two of these CTAs share
+// an SM, and beside one power of two of columns the other's are always left in one piece.)
 //
 // Every wait on an mbarrier is bounded; a wait that runs out sets an error bit and an abort flag, all roles fall
 // through to the common exit, outstanding copies are waited for and tensor memory is freed.
@@ -171,8 +179,8 @@ __device__ __forceinline__ void split_x(const float (&v)[8], uint32_t lane, uint
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
     // X = rn(x * 2^(22 - e)), e = exponent of the block's largest |x| plus one, so |X| <= 2^22; the unit of digit 0,
-    // with the half that a code counts, is 2^(e - 21): scale byte e - 21 + 127.  Blocks below 2^-104 keep the unit
-    // 2^-126; 2^127 and above count as infinite (scale byte 255, any digits).
+    // with the half that a code counts, is 2^(e - 21): scale byte e - 21 + 127.  Blocks below 2^-105 keep digit 0 at
+    // 2^-126, the unit of X at 2^-127; 2^127 and above count as infinite (scale byte 255, any digits).
     const uint32_t ex = top >> 23;                                // e = ex - 126
     const bool bad = ex >= 254u;
     const uint32_t unit = bad ? 1u : ex > 21u ? ex - 20u : 1u;    // scale byte of digit 0

@@ -8,8 +8,10 @@
 // One pass over x, bound by HBM: 2 or 4 bytes read and 17/32 byte written per value.  A warp takes segments of 256 columns
 // of a row, a lane 8 neighbouring columns of each (one 16-byte load of 16-bit values): the block maximum is two shuffles
 // over four lanes, the codes of a segment are 128 contiguous bytes, and its scales are two 4-byte words.  Where there is
-// work for it, four segments are under way at a time.  Measured: 2048 x 14336 bf16 14.4 us (5.2 TB/s), 8192 x 8192 bf16 29.9 us
-// (5.7 TB/s), fp32 44.4 us (6.9 TB/s).  The 16-bit types are near the rate at which their instructions issue, which is why
+// work for it, four segments are under way at a time.  Measured over buffers that rotate beyond L2 (in brackets: the same ones
+// again): 2048 x 14336 bf16 16.2 to 17.9 us (14.3 to 16.3), fp16 14.2 us (12.4), 8192 x 8192 bf16 30.4 us (5.6 TB/s), fp32 45.5 us
+// (6.7 TB/s: a stream of reads, which runs faster than a copy).  Rows that do not start at multiples of 16 bytes are read
+// value by value: 2048 rows of 14336, 14349 apart, bf16 27.3 us, fp16 26.5 us, fp32 34.6 us (aligned 20.9).  The 16-bit types are near the rate at which their instructions issue, which is why
 // maxima are taken two at a time and scales are turned over between lanes and stored four segments at once (17.2 -> 14.4 us).
 #include "axc_kernels.h"
 #include "axc_mx.cuh"

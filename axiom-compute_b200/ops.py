@@ -2,7 +2,11 @@
 
 torch is used for device memory and streams only; every function forwards raw device pointers
 and the current stream to ``libaxc_cuda.so``.  No function here computes anything itself and
-none has a CPU path: a non-CUDA tensor is an error.
+none has a CPU path: a non-CUDA tensor is an error.  Nothing is recorded for a backward pass:
+outputs do not require gradients, whatever the inputs do.
+
+Kernels report through `status` (``new_status``) only: bit 0 says that a bounded wait inside the
+kernel ran out and the output is not complete.  A call without `status` does not report it.
 """
 from __future__ import annotations
 
@@ -210,7 +214,9 @@ def _status_ptr(status: torch.Tensor, device: int) -> int:
 
 
 def mxfp4_scale_bytes(rows: int, n_blocks: int) -> int:
-    """Bytes of the scale tiles of an MXFP4 matrix (tiles of 128 rows x 4 blocks)."""
+    """Bytes of the scale tiles of an MXFP4 matrix (tiles of 128 rows x 4 blocks; the address of each byte is in
+    include/axc_cuda.h).  ``mxfp4_quantize`` writes all of them.  Whoever fills such a buffer otherwise sets the bytes
+    that belong to no row and block to zero: no call checks them, and a NaN scale there reaches the products."""
     return _tile_bytes(_count(rows, "rows"), _count(n_blocks, "n_blocks"))
 
 
@@ -280,8 +286,10 @@ def mxfp4_dequant(codes: torch.Tensor, scales: torch.Tensor, rows: int, n_blocks
 
 def mxfp4_matvec(codes: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, rows: int, n_blocks: int,
                  y: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None, m_tokens: int = 1) -> torch.Tensor:
-    """y[t, r] = sum_k W[r, k] x[t, k] with W in MXFP4, for 1 to 8 float32 vectors x of n_blocks * 32 values; x keeps
-    its precision (include/axc_cuda.h).  y has shape (rows,) for one vector, (m_tokens, rows) where x has more
+    """y[t, r] = sum_k W[r, k] x[t, k] with W in MXFP4, for 1 to 8 float32 vectors x of n_blocks * 32 values.  x is held
+    in fixed point, 23 bits with sign per block of 32: each value is off by at most 2^-22 of the block's largest |x|, so
+    small values beside a very large one lose bits that float32 has.  A block with a NaN, an infinity or a magnitude of
+    2^127 or more makes its token NaN.  y has shape (rows,) for one vector, (m_tokens, rows) where x has more
     dimensions than one or there are several."""
     device = _device_of(codes, "codes")
     rows, n_blocks, m_tokens = _count(rows, "rows"), _count(n_blocks, "n_blocks"), _count(m_tokens, "m_tokens", 1)
@@ -302,7 +310,9 @@ def mxfp4_prefill(w_codes: torch.Tensor, w_scales: torch.Tensor, a_codes: torch.
                   m_tokens: int, n_rows: int, n_blocks: int, c: Optional[torch.Tensor] = None,
                   status: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """C[m, n] = sum_k A[m, k] W[n, k] on the tensor cores, both operands in MXFP4 (tokens through
-    ``mxfp4_quantize``): C has shape (m_tokens, n_rows) in out_dtype, fp32 accumulation, one rounding."""
+    ``mxfp4_quantize``): C has shape (m_tokens, n_rows) in out_dtype, fp32 accumulation, one rounding.
+    The tensor cores' accumulation cuts off where fp32 addition rounds: an error of up to 2^-22 of sum |A W| per 64 columns
+    where scales lie far apart (include/axc_cuda.h)."""
     device = _device_of(w_codes, "w_codes")
     m_tokens, n_rows, n_blocks = _count(m_tokens, "m_tokens"), _count(n_rows, "n_rows"), _count(n_blocks, "n_blocks")
     wp, wsp = _codes_ptr(w_codes, n_rows, n_blocks, device, "w_codes"), _scales_ptr(w_scales, n_rows, n_blocks, device, "w_scales")
